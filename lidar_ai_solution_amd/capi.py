@@ -12,8 +12,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libscn_hip.so")
 
 OK = 0
-PRECISION_FP16, PRECISION_INT8 = 1, 2
-DTYPE_INT32, DTYPE_FP16, DTYPE_FP32, DTYPE_INT8 = 1, 2, 3, 7
+PRECISION_FP16, PRECISION_INT8, PRECISION_MXFP4 = 1, 2, 3
+DTYPE_INT32, DTYPE_FP16, DTYPE_FP32, DTYPE_INT8, DTYPE_MXFP4 = 1, 2, 3, 7, 16
 ORDER_XYZ, ORDER_ZYX = 1, 2
 BUILD_SORTMASK, BUILD_AUX_STREAM, BUILD_KEEP_ALL, BUILD_TILE_PLANS = 1, 4, 256, 512
 
@@ -47,6 +47,14 @@ class ConvIO(C.Structure):
                 ("res_dtype", C.c_int), ("res_dynamic_range", C.c_float), ("res_ld", u32), ("mid_dtype", C.c_int),
                 ("mid_dynamic_range", C.c_float), ("a_requant_range", C.c_float), ("b_requant_range", C.c_float),
                 ("relu_after_add", C.c_int), ("fixed_launch_points", u32)]
+
+
+class MxProductIO(C.Structure):
+    _fields_ = [("a_dev", vp), ("a_dtype", C.c_int), ("a_ld", u32), ("a_scales_dev", vp), ("a_scales_ld", u32),
+                ("b_codes_dev", vp), ("b_codes_ld", u32), ("b_scales_dev", vp), ("b_scales_ld", u32), ("m", u32), ("n", u32),
+                ("k", u32), ("m_dev", vp), ("bias_dev", vp), ("bias_dtype", C.c_int), ("relu", C.c_int), ("res_dev", vp),
+                ("res_dtype", C.c_int), ("res_ld", u32), ("relu_after_add", C.c_int), ("out_dev", vp),
+                ("out_dtype", C.c_int), ("out_ld", u32), ("workspace_dev", vp), ("workspace_bytes", C.c_size_t)]
 
 
 class TensorView(C.Structure):
@@ -102,6 +110,12 @@ _SIGNATURES = {
     "scn_convert_rows": (C.c_int, [vp, C.c_int, u32, u32, C.c_float, vp, C.c_int, u32, u32, C.c_float, C.c_int, u32, vp, vp]),
     "scn_add_relu": (C.c_int, [vp, C.c_int, C.c_float, C.c_float, vp, C.c_int, C.c_float, C.c_float, vp, C.c_int,
                                C.c_float, C.c_int, u32, u32, vp, vp]),
+    "scn_mx_row_bytes": (C.c_size_t, [u32]),
+    "scn_mx_quantize_rows": (C.c_int, [vp, C.c_int, u32, u32, C.c_float, C.c_int, vp, u32, vp, u32, u32, vp, vp]),
+    "scn_mx_dequantize_rows": (C.c_int, [vp, u32, vp, u32, u32, vp, C.c_int, u32, u32, vp, vp]),
+    "scn_mx_product_direct_rows": (u32, []),
+    "scn_mx_product_workspace": (C.c_size_t, [u32, u32]),
+    "scn_mx_product": (C.c_int, [C.POINTER(MxProductIO), vp]),
     "scn_scatter_dense": (C.c_int, [vp, C.c_int, C.c_float, u32, u32, vp, u32, vp, i5, vp, vp, vp]),
     "scn_scatter_dense_layout": (C.c_int, [vp, C.c_int, C.c_float, u32, u32, vp, u32, vp, i5, vp, C.c_int, C.c_int,
                                            C.c_int, C.c_float, vp, vp]),

@@ -1,6 +1,7 @@
 // Host side of the convolution: weight packing into MFMA operand order, argument checks and the
 // choice of kernel; C ABI of the convolution stage.
 #include "scn_conv_args.hpp"
+#include "scn_mx.hpp"
 
 #include <algorithm>
 #include <cstdlib>
@@ -19,6 +20,7 @@ bool ConvWeights::init(const uint16_t* w_fp16, const int shape[5], const float* 
     set_error("int8 convolution needs weight_dynamic_ranges");
     return false;
   }
+  if (prec == SCN_PRECISION_MXFP4) return init_mx(w_fp16, bias_fp16);
   const int epc = prec == SCN_PRECISION_INT8 ? 16 : 8;  // elements per 16-byte chunk
   const int cout_pad = mtiles * 16;
   std::vector<float> ws(cout_pad, 1.f), bs(cout_pad, 0.f);
@@ -94,12 +96,40 @@ bool ConvWeights::init(const uint16_t* w_fp16, const int shape[5], const float* 
   return true;
 }
 
+// Weights of a convolution on microscaled rows, in the operand order of the 32x32 scaled matrix instruction: lane l of
+// fragment (step s, tile t) is output channel 32 t + l % 32, block 2 s + l / 32 of the sequence (offset, block of the row).
+bool ConvWeights::init_mx(const uint16_t* w_fp16, const uint16_t* bias_fp16) {
+  std::vector<uint8_t> frag((size_t)steps * mtiles32 * 64 * 16, 0), sc((size_t)steps * mtiles32 * 64, 0);
+  std::vector<float> bs((size_t)mtiles32 * 32, 0.f);
+  if (bias_fp16)
+    for (int c = 0; c < cout; ++c) bs[c] = half_bits_to_float(bias_fp16[c]);
+  float v[32];
+  for (int s = 0; s < steps; ++s)
+    for (int t = 0; t < mtiles32; ++t)
+      for (int l = 0; l < 64; ++l) {
+        const int g = 2 * s + l / 32, k = g / chunks, b = g % chunks, co = 32 * t + l % 32;
+        if (k >= kvol || co >= cout) continue;
+        const int nv = cin - 32 * b < 32 ? cin - 32 * b : 32;
+        for (int i = 0; i < nv; ++i) v[i] = half_bits_to_float(w_fp16[((size_t)co * kvol + k) * cin + 32 * b + i]);
+        const size_t f = ((size_t)s * mtiles32 + t) * 64 + l;
+        sc[f] = mx_quantize_block(v, nv, &frag[f * 16]);
+      }
+  if (!wfrag.alloc(frag.size()) || !wscale.alloc(sc.size()) || !bias.alloc(bs.size() * 4)) return false;
+  if (hipMemcpy(wfrag.p, frag.data(), frag.size(), hipMemcpyHostToDevice) != hipSuccess ||
+      hipMemcpy(wscale.p, sc.data(), sc.size(), hipMemcpyHostToDevice) != hipSuccess ||
+      hipMemcpy(bias.p, bs.data(), bs.size() * 4, hipMemcpyHostToDevice) != hipSuccess) {
+    set_error("weight upload failed");
+    return false;
+  }
+  return true;
+}
+
 bool conv_tile_covers(const ConvWeights& w) {
   static const bool off = [] {
     const char* e = getenv("SCN_CONV_IMPL");
     return e && (!strcmp(e, "lds") || !strcmp(e, "rows"));
   }();
-  if (off || w.kvol > 31 || w.mtiles32 < 1 || w.mtiles32 > 2) return false;
+  if (off || w.precision == SCN_PRECISION_MXFP4 || w.kvol > 31 || w.mtiles32 < 1 || w.mtiles32 > 2) return false;
   if (w.chunks != 1 && w.chunks != 2 && w.chunks != 4) return false;
   // the whole weight tensor stays in LDS: [steps32][mtiles32] fragments of 1 KB
   return (size_t)w.steps32 * w.mtiles32 * 1024 + 512 <= 60 * 1024;
@@ -108,7 +138,7 @@ bool conv_tile_covers(const ConvWeights& w) {
 int conv_forward(const ConvWeights& w, const int32_t* nbr, uint32_t nbr_ld, const uint32_t* n_out_dev,
                  uint32_t n_bound, uint32_t n_hint, const scn_conv_io& io, hipStream_t stream, const PlanView* plan) {
   if (n_bound == 0) return SCN_OK;
-  const int esz = w.precision == SCN_PRECISION_INT8 ? 1 : 2;
+  const int esz = w.precision == SCN_PRECISION_FP16 ? 2 : 1;   // (microscaled rows: x_ld is in bytes)
   SCN_REQUIRE(io.x_dev && io.out_dev, SCN_ERR_INVALID, "conv: null input or output");
   SCN_REQUIRE(io.x_ld >= w.cin_pad, SCN_ERR_INVALID, "conv: input row stride %u < padded channels %u", io.x_ld,
               w.cin_pad);
@@ -185,8 +215,9 @@ int conv_forward(const ConvWeights& w, const int32_t* nbr, uint32_t nbr_ld, cons
   // whichever is more
   a.launch_rows = io.fixed_launch_points ? std::min(n_bound, std::max(io.fixed_launch_points, n_hint)) : n_bound;
   if (a.launch_rows == 0) a.launch_rows = 1;
-  const bool ok = w.precision == SCN_PRECISION_INT8 ? conv_dispatch_int8(w, n_hint, a, stream)
-                                                    : conv_dispatch_fp16(w, n_hint, a, stream);
+  const bool ok = w.precision == SCN_PRECISION_INT8    ? conv_dispatch_int8(w, n_hint, a, stream)
+                  : w.precision == SCN_PRECISION_MXFP4 ? conv_dispatch_mx(w, n_hint, a, stream)
+                                                       : conv_dispatch_fp16(w, n_hint, a, stream);
   SCN_REQUIRE(ok, SCN_ERR_UNSUPPORTED, "conv: no kernel for Cin=%d Cout=%d (chunks %d, m-tiles %d)", w.cin, w.cout,
               w.chunks, w.mtiles);
   SCN_HIP(hipGetLastError());
@@ -202,7 +233,8 @@ extern "C" {
 
 scn_conv* scn_conv_create(const uint16_t* weight_fp16, const int weight_shape[5], const float* weight_dynamic_ranges,
                           const uint16_t* bias_fp16, int precision) {
-  if (!weight_fp16 || !weight_shape || (precision != SCN_PRECISION_FP16 && precision != SCN_PRECISION_INT8)) {
+  if (!weight_fp16 || !weight_shape || (precision != SCN_PRECISION_FP16 && precision != SCN_PRECISION_INT8 &&
+                                           precision != SCN_PRECISION_MXFP4)) {
     set_error("scn_conv_create: invalid arguments");
     return nullptr;
   }

@@ -63,6 +63,7 @@ struct PlanView {
 // n_hint: expected number of output rows.  Returns false when no kernel covers the shape.
 bool conv_dispatch_int8(const ConvWeights& w, uint32_t n_hint, ConvArgs& a, hipStream_t stream);
 bool conv_dispatch_fp16(const ConvWeights& w, uint32_t n_hint, ConvArgs& a, hipStream_t stream);
+bool conv_dispatch_mx(const ConvWeights& w, uint32_t n_hint, ConvArgs& a, hipStream_t stream);
 // Shapes the tile-plan kernel covers (narrow layers: input rows of at most 64 bytes, at most 64 output channels).
 bool conv_tile_covers(const ConvWeights& w);
 

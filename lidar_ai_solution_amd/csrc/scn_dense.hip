@@ -1,5 +1,6 @@
 // Elementwise glue (quantise / dequantise / pad, add + relu) and sparse -> dense of the SCN path (gfx950).
 #include "scn_device.hpp"
+#include "scn_mx.hpp"
 #include <mutex>
 
 #include <algorithm>
@@ -46,6 +47,14 @@ __global__ __launch_bounds__(256) void k_convert_rows(const void* in, int in_dty
 int convert_rows(const void* in, int in_dtype, uint32_t in_c, uint32_t in_ld, float in_range, void* out,
                  int out_dtype, uint32_t out_c, uint32_t out_ld, float out_range, int relu, uint32_t n,
                  const uint32_t* n_dev, hipStream_t stream) {
+  if (out_dtype == SCN_DTYPE_MXFP4) {   // one-buffer microscaled rows: the scales follow the codes of their row
+    SCN_REQUIRE(in_c > 0 && out_ld >= mx_row_bytes(in_c), SCN_ERR_INVALID,
+                "convert_rows: a microscaled row of %u channels needs %u bytes (stride %u)", in_c, mx_row_bytes(in_c), out_ld);
+    SCN_REQUIRE(out || n == 0, SCN_ERR_INVALID, "convert_rows: null output");
+    uint8_t* codes = static_cast<uint8_t*>(out);
+    return mx_quantize_rows(in, in_dtype, in_c, in_ld, in_range, relu, codes, out_ld, codes + mx_blocks(in_c) * kMxBlockBytes,
+                            out_ld, n, n_dev, stream);
+  }
   const float in_scale = in_range > 0.f ? in_range / 127.f : 1.f;
   const float out_scale = out_range > 0.f ? 127.f / out_range : 1.f;
   if (n == 0) return SCN_OK;

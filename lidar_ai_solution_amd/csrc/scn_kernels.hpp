@@ -123,17 +123,18 @@ struct Rulebook {
 struct ConvWeights {
   int cin = 0, cout = 0, kvol = 0, ks[3] = {1, 1, 1};
   int precision = SCN_PRECISION_FP16;  // compute precision
-  int chunks = 0;   // 16-byte chunks per (padded) input row
+  int chunks = 0;   // 16-byte chunks per (padded) input row; MXFP4: blocks of 32 channels per input row
   int mtiles = 0;   // ceil(cout / 16)
   int steps = 0;    // MFMA K-steps = ceil(kvol * chunks / 4)
-  uint32_t cin_pad = 0;  // padded input channels the kernel expects (elements)
-  DevBuf wfrag;     // [steps][mtiles][64] x 16 bytes, MFMA A-operand order
+  uint32_t cin_pad = 0;  // padded input channels the kernel expects (elements); MXFP4: bytes of an input row
+  DevBuf wfrag;     // [steps][mtiles][64] x 16 bytes, MFMA A-operand order (MXFP4: 32x32 tiles, ceil(cout / 32) of them)
   int mtiles32 = 0, steps32 = 0;
   DevBuf zrow;      // 512 bytes of zeros, then 64 words of -1
   DevBuf wfrag32;   // cout > 16: [steps32][mtiles32][64] x 16 bytes, A-operand order of the 32x32 MFMA
-  DevBuf wscale;    // fp32 [cout_pad]: s_w[c] (int8) or 1
+  DevBuf wscale;    // fp32 [cout_pad]: s_w[c] (int8) or 1; MXFP4: scale bytes [steps][tiles][64]
   DevBuf bias;      // fp32 [cout_pad]
   bool init(const uint16_t* w_fp16, const int shape[5], const float* ranges, const uint16_t* bias_fp16, int prec);
+  bool init_mx(const uint16_t* w_fp16, const uint16_t* bias_fp16);   // MXFP4 packing, after set_geometry
   // the sizes above from a weight shape [Cout, K0, K1, K2, Cin] (host only; false for a shape with a dimension < 1)
   bool set_geometry(const int shape[5], int prec) {
     cout = shape[0];
@@ -144,15 +145,21 @@ struct ConvWeights {
     if (cout <= 0 || cin <= 0 || ks[0] <= 0 || ks[1] <= 0 || ks[2] <= 0) return false;
     kvol = ks[0] * ks[1] * ks[2];
     precision = prec;
+    mtiles = (cout + 15) / 16;
+    mtiles32 = (cout + 31) / 32;
+    if (prec == SCN_PRECISION_MXFP4) {
+      chunks = (cin + 31) / 32;
+      cin_pad = (uint32_t)((chunks * 16 + ((chunks + 3) & ~3) + 15) & ~15);   // one-buffer row: codes, then scales
+      steps = steps32 = (kvol * chunks + 1) / 2;                             // two blocks per matrix instruction
+      return true;
+    }
     const int epc = prec == SCN_PRECISION_INT8 ? 16 : 8;  // elements per 16-byte chunk
     const int ch = (cin + epc - 1) / epc;
     int p2 = 1;
     while (p2 < ch) p2 <<= 1;  // chunks per row rounded to a power of two (rows are padded to it)
     chunks = p2;
     cin_pad = (uint32_t)(chunks * epc);
-    mtiles = (cout + 15) / 16;
     steps = (kvol * chunks + 3) / 4;
-    mtiles32 = (cout + 31) / 32;
     if (mtiles32 == 3) mtiles32 = 4;  // kernels exist for 1, 2 and 4 tiles; the fourth is zero weights
     steps32 = 4 * ((kvol * chunks + 7) / 8);  // whole iterations of 4 K-steps, zero weights beyond the volume
     return true;

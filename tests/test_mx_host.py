@@ -1,0 +1,104 @@
+"""Microscaled rows without a GPU: the format's oracle against tables written out by hand, layout sizes, refusals."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from lidar_ai_solution_amd import capi
+from tests import mx_reference as R
+
+GOOD = 1 << 20   # an aligned address that no refused call reads
+
+
+def test_reference_rounds_like_the_table():
+    """One block whose largest magnitude is 6 (scale 1): every level, every midpoint (ties to the even code), both signs."""
+    v = [0, .25, .2500001, .5, .75, 1, 1.25, 1.2500001, 1.5, 1.75, 2, 2.5, 2.500001, 3, 3.5, 4, 5, 5.000001, 6, -0.0, -.25, -.75, -5, -6]
+    want = [0, 0, 1, 1, 2, 2, 2, 3, 3, 4, 4, 4, 5, 5, 6, 6, 6, 7, 7, 8, 8, 10, 14, 15]
+    codes, scales = R.quantize(np.array([v]))
+    got = np.stack([codes & 15, codes >> 4], 2).reshape(1, -1)[0, :len(v)]
+    assert got.tolist() == want and scales.tolist() == [[127, 0, 0, 0]]
+
+
+@pytest.mark.parametrize("top, byte, code", [(7.9, 127, 7), (8.0, 128, 6), (2.0 ** 127, 252, 6), (2.0 ** -125, 0, 6),
+                                             (2.0 ** -127, 0, 2), (2.0 ** -149, 0, 0), (0.0, 0, 0)])
+def test_reference_scales(top, byte, code):
+    codes, scales = R.quantize(np.array([[top]]))
+    assert (int(scales[0, 0]), int(codes[0, 0])) == (byte, code)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_reference_marks_blocks_that_are_not_finite(bad):
+    x = np.ones((1, 70))
+    x[0, 40] = bad
+    codes, scales = R.quantize(x)
+    assert scales[0].tolist() == [125, 255, 125, 0] and not codes[0, 16:32].any()
+    v = R.values(codes, scales, 70)
+    assert np.isnan(v[0, 32:64]).all() and (np.delete(v[0], np.s_[32:64]) == 1).all()
+
+
+def test_row_bytes():
+    L = capi.lib()
+    for c in range(1, 600):
+        blocks = -(-c // 32)
+        assert L.scn_mx_row_bytes(c) == -(-(16 * blocks + -(-blocks // 4) * 4) // 16) * 16
+    assert L.scn_mx_product_workspace(16, 64) == 0
+    assert L.scn_mx_product_workspace(17, 64) == 17 * L.scn_mx_row_bytes(64)
+
+
+def _quantize(**over):
+    a = dict(x=GOOD, dtype=capi.DTYPE_FP16, c=64, ld=64, rng=0.0, relu=0, codes=GOOD, cl=32, scales=GOOD, sl=4, n=5)
+    a.update(over)
+    return capi.lib().scn_mx_quantize_rows(a["x"], a["dtype"], a["c"], a["ld"], a["rng"], a["relu"], a["codes"], a["cl"],
+                                           a["scales"], a["sl"], a["n"], None, None)
+
+
+@pytest.mark.parametrize("over", [dict(x=None), dict(x=GOOD + 1), dict(dtype=capi.DTYPE_INT32), dict(dtype=capi.DTYPE_INT8), dict(c=0),
+                                  dict(ld=63), dict(codes=None), dict(codes=GOOD + 8), dict(cl=16), dict(cl=40), dict(scales=None),
+                                  dict(scales=GOOD + 2), dict(sl=2), dict(sl=6), dict(c=160, ld=160, cl=80, sl=4)])
+def test_quantize_refusals(over):
+    assert _quantize(**over) == 1
+    assert b"mx_quantize_rows" in capi.lib().scn_last_error()
+
+
+def test_no_rows_is_no_work():
+    assert _quantize(n=0, x=None) == 0
+    L = capi.lib()
+    assert L.scn_mx_dequantize_rows(None, 0, None, 0, 64, None, capi.DTYPE_FP16, 64, 0, None, None) == 0
+    assert L.scn_mx_product(C.byref(_io(m=0, a_dev=None)), None) == 0
+
+
+@pytest.mark.parametrize("over", [dict(out=None), dict(out=GOOD + 1), dict(dtype=capi.DTYPE_INT8), dict(ld=63), dict(codes=None), dict(cl=24)])
+def test_dequantize_refusals(over):
+    a = dict(codes=GOOD, cl=32, scales=GOOD, sl=4, c=64, out=GOOD, dtype=capi.DTYPE_FP16, ld=64)
+    a.update(over)
+    assert capi.lib().scn_mx_dequantize_rows(a["codes"], a["cl"], a["scales"], a["sl"], a["c"], a["out"], a["dtype"], a["ld"], 5,
+                                             None, None) == 1
+    assert b"mx_dequantize_rows" in capi.lib().scn_last_error()
+
+
+def _io(**over):
+    io = capi.MxProductIO()
+    base = dict(a_dev=GOOD, a_dtype=capi.DTYPE_MXFP4, a_ld=32, a_scales_dev=GOOD, a_scales_ld=4, b_codes_dev=GOOD, b_codes_ld=32,
+                b_scales_dev=GOOD, b_scales_ld=4, m=40, n=24, k=64, out_dev=GOOD, out_dtype=capi.DTYPE_FP16, out_ld=24)
+    base.update(over)
+    for key, v in base.items():
+        setattr(io, key, v)
+    return io
+
+
+@pytest.mark.parametrize("over", [dict(a_dev=None), dict(a_dtype=capi.DTYPE_INT8), dict(a_ld=16), dict(a_scales_dev=None), dict(b_codes_dev=None),
+                                  dict(b_codes_ld=24), dict(b_scales_ld=3), dict(n=0), dict(k=0), dict(out_dev=None), dict(out_dev=GOOD + 1),
+                                  dict(out_dtype=capi.DTYPE_INT8), dict(out_ld=23), dict(bias_dev=GOOD, bias_dtype=capi.DTYPE_INT8),
+                                  dict(bias_dev=GOOD + 2, bias_dtype=capi.DTYPE_FP32), dict(res_dev=GOOD, res_dtype=0),
+                                  dict(res_dev=GOOD, res_dtype=capi.DTYPE_FP16, res_ld=23), dict(a_dtype=capi.DTYPE_FP16, a_ld=63),
+                                  dict(a_dtype=capi.DTYPE_FP16, a_ld=64), dict(a_dtype=capi.DTYPE_FP32, a_ld=64, workspace_dev=GOOD, workspace_bytes=1919),
+                                  dict(a_dtype=capi.DTYPE_FP32, a_ld=64, workspace_dev=GOOD + 8, workspace_bytes=1 << 20)])
+def test_product_refusals(over):
+    assert capi.lib().scn_mx_product(C.byref(_io(**over)), None) == 1
+    assert b"mx_product" in capi.lib().scn_last_error()
+
+
+def test_conversion_to_microscaled_rows_refuses_short_rows():
+    L = capi.lib()
+    assert L.scn_convert_rows(GOOD, capi.DTYPE_FP16, 64, 64, 0.0, GOOD, capi.DTYPE_MXFP4, 0, 47, 0.0, 0, 5, None, None) == 1
+    assert b"needs 48 bytes" in L.scn_last_error()
