@@ -19,7 +19,7 @@
 namespace bevfusion {
 namespace lidar {
 
-enum class Precision : int { NonePrecision = 0, Float16 = 1, Int8 = 2 };
+enum class Precision : int { NonePrecision = 0, Float16 = 1, Int8 = 2, MxFp4 = 3 };
 
 struct SCNParameter {
   VoxelizationParameter voxelization;

@@ -21,7 +21,7 @@
 namespace spconv {
 
 enum class DType : int { None = 0, Int32 = 1, Float16 = 2 };
-enum class Precision : int { None = 0, Float16 = 1, Int8 = 2 };
+enum class Precision : int { None = 0, Float16 = 1, Int8 = 2, MxFp4 = 3 };
 
 class DTensor {
  public:
@@ -188,6 +188,7 @@ inline const char* get_precision_string(Precision precision) {
   switch (precision) {
     case Precision::Float16: return "Float16";
     case Precision::Int8: return "Int8";
+    case Precision::MxFp4: return "MxFp4";
     default: return "None";
   }
 }

@@ -26,7 +26,8 @@ namespace spconv {
 
 #define Exported __attribute__((visibility("default")))
 
-enum class Precision : int { None = 0, Float16 = 1, Int8 = 2 };
+// MxFp4 is not in the reference: convolutions on microscaled 4-bit rows (SCN_PRECISION_MXFP4).
+enum class Precision : int { None = 0, Float16 = 1, Int8 = 2, MxFp4 = 3 };
 enum class TensorLayout : int { None = 0, NCHW = 1, NCHW32 = 2, NHWzC = 3 };
 enum class LoggerLevel : int { Verb = 0, Warn = 1, Error = 2, Quiet = 99 };
 
@@ -50,6 +51,7 @@ inline const char* get_precision_string(Precision precision) {
   switch (precision) {
     case Precision::Float16: return "Float16";
     case Precision::Int8: return "Int8";
+    case Precision::MxFp4: return "MxFp4";
     default: return "None";
   }
 }

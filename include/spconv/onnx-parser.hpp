@@ -14,7 +14,8 @@ namespace spconv {
 /**
  * onnx_file: the custom "scn" ONNX dialect written by the reference's exporters.
  * precision: Float16 forces every layer to fp16; Int8 honours the per-layer precision attributes
- *            (layers without dynamic ranges stay fp16).
+ *            (layers without dynamic ranges stay fp16); MxFp4 runs the convolutions marked int8 or mxfp4 on microscaled
+ *            4-bit rows and everything else in fp16.
  * sortmask: a hint, passed on (the engine re-orders rows only where that is faster; results never change).
  * with_auxiliary_stream: passed on (rulebooks are built on a second stream ahead of the convolutions).
  * enable_blackwell: accepted for source compatibility, ignored.

@@ -247,6 +247,13 @@ static Plan make_plan(const std::vector<NodeDesc>& nodes, size_t ntensors, int e
   for (size_t i = 0; i < nodes.size(); ++i) {
     const NodeDesc& n = nodes[i];
     for (size_t s = 0; s < n.in.size(); ++s) p.consumers[n.in[s]].push_back({(int)i, (int)s});
+    // An MXFP4 engine runs the convolutions that the model marks for low precision (int8 or mxfp4) on microscaled rows;
+    // their scales come with the rows, so no dynamic ranges are needed.  Every tensor stays fp16.
+    if (engine_precision == SCN_PRECISION_MXFP4) {
+      if (n.op == Op::Conv && (n.precision == SCN_PRECISION_INT8 || n.precision == SCN_PRECISION_MXFP4))
+        p.comp[i] = SCN_PRECISION_MXFP4;
+      continue;
+    }
     if (engine_precision != SCN_PRECISION_INT8) {
       if ((n.op == Op::Conv || n.op == Op::Add) && n.precision == SCN_PRECISION_INT8)
         SCN_LOGV("Ignore the layer[%s] precision[int8] because the model precision configured fp16", n.name.c_str());
@@ -254,7 +261,9 @@ static Plan make_plan(const std::vector<NodeDesc>& nodes, size_t ntensors, int e
     }
     if (n.op == Op::Conv) {
       const bool ok = n.in_range > 0.f && (int)n.wranges.size() == n.wshape[0];
-      p.comp[i] = (n.precision == SCN_PRECISION_INT8 && ok) ? SCN_PRECISION_INT8 : SCN_PRECISION_FP16;
+      p.comp[i] = n.precision == SCN_PRECISION_MXFP4            ? SCN_PRECISION_MXFP4
+                  : (n.precision == SCN_PRECISION_INT8 && ok) ? SCN_PRECISION_INT8
+                                                              : SCN_PRECISION_FP16;
       p.outp[i] = n.out_precision == SCN_PRECISION_INT8 ? SCN_PRECISION_INT8 : SCN_PRECISION_FP16;
     } else if (n.op == Op::Add) {
       const bool ok = n.a_range > 0.f && n.b_range > 0.f;
@@ -496,10 +505,14 @@ static bool build_engine(scn_engine& e) {
         st.coord = x.coord;
         st.coord_out = slot.coord_out;
         st.t_in = n.in[0];
-        const int want_dtype = comp == SCN_PRECISION_INT8 ? SCN_DTYPE_INT8 : SCN_DTYPE_FP16;
+        const int want_dtype = comp == SCN_PRECISION_INT8    ? SCN_DTYPE_INT8
+                               : comp == SCN_PRECISION_MXFP4 ? SCN_DTYPE_MXFP4
+                                                             : SCN_DTYPE_FP16;
         float want_range = 0.f;
         bool need_convert = false;
-        if (comp == SCN_PRECISION_INT8) {
+        if (comp == SCN_PRECISION_MXFP4) {
+          need_convert = true;  // rows in the one-buffer microscaled form, cin_pad bytes each
+        } else if (comp == SCN_PRECISION_INT8) {
           if (x.dtype == SCN_DTYPE_INT8) {
             st.x_range = x.range;
           } else {
@@ -532,7 +545,7 @@ static bool build_engine(scn_engine& e) {
             Step cs;
             cs.kind = StepKind::Convert;
             cs.node = (int)i;
-            cs.label = std::string(want_dtype == SCN_DTYPE_INT8 ? "quantize(" : (xx.dtype == SCN_DTYPE_INT8 ? "dequantize(" : "pad(")) +
+            cs.label = std::string(want_dtype == SCN_DTYPE_INT8 || want_dtype == SCN_DTYPE_MXFP4 ? "quantize(" : (xx.dtype == SCN_DTYPE_INT8 ? "dequantize(" : "pad(")) +
                        e.tdesc[n.in[0]].name + ")";
             cs.t_in = n.in[0];
             cs.t_out = cvi;
@@ -915,7 +928,7 @@ static int allocate_runtime(scn_engine& e) {
     std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return born[a] < born[b]; });
     for (int t : order) {
       const RtTensor& x = e.tensors[t];
-      const size_t bytes = ((size_t)e.coords[x.coord].cap * x.ld * (x.dtype == SCN_DTYPE_INT8 ? 1 : 2) + 255) & ~(size_t)255;
+      const size_t bytes = ((size_t)e.coords[x.coord].cap * x.ld * (x.dtype == SCN_DTYPE_FP16 ? 2 : 1) + 255) & ~(size_t)255;
       int best = -1;
       for (size_t k = 0; k < pool.size(); ++k)   // the free block that is closest in size
         if (pool[k].busy_until < born[t]) {
@@ -961,7 +974,7 @@ static int allocate_runtime(scn_engine& e) {
       continue;
     }
     const size_t rows = e.coords[x.coord].cap;
-    const size_t bytes = rows * x.ld * (x.dtype == SCN_DTYPE_INT8 ? 1 : 2);
+    const size_t bytes = rows * x.ld * (x.dtype == SCN_DTYPE_FP16 ? 2 : 1);
     if (x.buf.bytes < bytes) {
       if (!x.buf.alloc(bytes)) return SCN_ERR_HIP;
       SCN_HIP(hipMemset(x.buf.p, 0, bytes));
@@ -1557,8 +1570,8 @@ int scn_builder_push_output(scn_builder* b, int tensor) {
 scn_engine* scn_builder_build(scn_builder* b, int precision, unsigned flags, void* stream) {
   (void)stream;
   if (!b) return nullptr;
-  if (precision != SCN_PRECISION_FP16 && precision != SCN_PRECISION_INT8) {
-    set_error("build: precision must be Float16 (1) or Int8 (2)");
+  if (precision != SCN_PRECISION_FP16 && precision != SCN_PRECISION_INT8 && precision != SCN_PRECISION_MXFP4) {
+    set_error("build: precision must be Float16 (1), Int8 (2) or MxFp4 (3)");
     return nullptr;
   }
   auto* e = new scn_engine();
@@ -1573,7 +1586,7 @@ scn_engine* scn_builder_build(scn_builder* b, int precision, unsigned flags, voi
     return nullptr;
   }
   SCN_LOGV("engine built: %zu nodes -> %zu steps, %zu rulebooks, precision %s", e->nodes.size(), e->steps.size(),
-           e->rulebooks.size(), precision == SCN_PRECISION_INT8 ? "int8" : "fp16");
+           e->rulebooks.size(), precision == SCN_PRECISION_INT8 ? "int8" : precision == SCN_PRECISION_MXFP4 ? "mxfp4" : "fp16");
   return e;
 }
 
@@ -1688,6 +1701,7 @@ static scn_engine* create_from_model_bytes(const std::string& bytes, const char*
   auto prec_of = [&](const OnnxNode& n, const char* attr) {
     const OnnxAttr* a = n.find(attr);
     int p = (a && a->s == "int8") ? SCN_PRECISION_INT8 : SCN_PRECISION_FP16;
+    if (a && a->s == "mxfp4" && n.op_type == "SparseConvolution" && !strcmp(attr, "precision")) p = SCN_PRECISION_MXFP4;
     const bool is_output = !strcmp(attr, "output_precision");
     for (int i = 0; i < n_overrides; ++i) {
       const scn_precision_override& o = overrides[i];
@@ -1698,6 +1712,7 @@ static scn_engine* create_from_model_bytes(const std::string& bytes, const char*
       if (subject != o.selector && !add_alias) continue;
       const int v = is_output ? o.output_precision : o.precision;
       if (v == SCN_PRECISION_FP16 || v == SCN_PRECISION_INT8) p = v;
+      if (v == SCN_PRECISION_MXFP4 && !is_output && n.op_type == "SparseConvolution") p = v;
     }
     return p;
   };

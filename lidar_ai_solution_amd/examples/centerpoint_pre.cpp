@@ -2,7 +2,7 @@
 // raw fp32 sweep -> PreProcessCuda::generateVoxels / getOutput (include/legacy/preprocess.h) -> the older
 // single-call engine interface (include/legacy/spconv/engine.hpp) -> dense BEV tensor.
 //
-//   centerpoint_pre <model.scn.onnx> <points.bin: fp32 [N, 5]> [fp16|int8] [output prefix]
+//   centerpoint_pre <model.scn.onnx> <points.bin: fp32 [N, 5]> [fp16|int8|mxfp4] [output prefix]
 // writes <prefix>.features.tensor / <prefix>.indices.tensor (the voxels) and <prefix>.bev.tensor
 #include <hip/hip_runtime.h>
 
@@ -18,10 +18,12 @@
 
 int main(int argc, char** argv) {
   if (argc < 3) {
-    printf("usage: %s model.onnx points.bin [fp16|int8] [output prefix]\n", argv[0]);
+    printf("usage: %s model.onnx points.bin [fp16|int8|mxfp4] [output prefix]\n", argv[0]);
     return 1;
   }
-  const auto precision = (argc > 3 && !strcmp(argv[3], "int8")) ? spconv::Precision::Int8 : spconv::Precision::Float16;
+  const auto precision = (argc > 3 && !strcmp(argv[3], "int8"))    ? spconv::Precision::Int8
+                         : (argc > 3 && !strcmp(argv[3], "mxfp4")) ? spconv::Precision::MxFp4
+                                                                  : spconv::Precision::Float16;
   const std::string prefix = argc > 4 ? argv[4] : "centerpoint";
   FILE* f = fopen(argv[2], "rb");
   if (!f) {

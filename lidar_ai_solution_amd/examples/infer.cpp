@@ -12,7 +12,7 @@
 // Switches come from the environment so that the positional command line stays what it was:
 //   SCN_USE_HIPGRAPH=1  SCN_USE_DDS=1  SCN_SORTMASK=1  SCN_AUX_STREAM=1  SCN_FIXED_LAUNCH_POINTS=<n>  SCN_SEED=<n>
 //
-//   infer <model.scn.onnx> <features.tensor> <indices.tensor> <g0> <g1> <g2> [fp16|int8] [output prefix]
+//   infer <model.scn.onnx> <features.tensor> <indices.tensor> <g0> <g1> <g2> [fp16|int8|mxfp4] [output prefix]
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -228,13 +228,15 @@ static int search_best_perf(Task& t, hipStream_t stream) {
 
 int main(int argc, char** argv) {
   if (argc < 7) {
-    printf("usage: %s model.onnx features.tensor indices.tensor g0 g1 g2 [fp16|int8] [output prefix]\n", argv[0]);
+    printf("usage: %s model.onnx features.tensor indices.tensor g0 g1 g2 [fp16|int8|mxfp4] [output prefix]\n", argv[0]);
     printf("spconv-compatible API %s on %s\n", NVSPCONV_VERSION, SCN_BACKEND);
     return 1;
   }
   Task t;
   t.onnx = argv[1];
-  t.precision = (argc > 7 && !strcmp(argv[7], "int8")) ? spconv::Precision::Int8 : spconv::Precision::Float16;
+  t.precision = (argc > 7 && !strcmp(argv[7], "int8"))    ? spconv::Precision::Int8
+                : (argc > 7 && !strcmp(argv[7], "mxfp4")) ? spconv::Precision::MxFp4
+                                                         : spconv::Precision::Float16;
   if (argc > 8) t.out_prefix = argv[8];
   t.grid = {atoi(argv[4]), atoi(argv[5]), atoi(argv[6])};
   t.use_graph = env_is_1("SCN_USE_HIPGRAPH");

@@ -3,7 +3,7 @@
 // what the reference cannot do there: voxelization and backbone captured together into ONE HIP graph (no host
 // round trip between them) and replayed on frames of different sizes.
 //
-//   lidar_scn <model.scn.onnx> <points.tensor fp16 [N, F]> <xyz|zyx> <fp16|int8> <output prefix> [aux]
+//   lidar_scn <model.scn.onnx> <points.tensor fp16 [N, F]> <xyz|zyx> <fp16|int8|mxfp4> <output prefix> [aux]
 //
 // Runs the full frame eagerly and saves it to <prefix>.eager.tensor, then captures one forward and replays the
 // graph on frames of N, N/2, N/3 and N points, comparing every replay with an eager forward of the same points.
@@ -32,7 +32,7 @@ static std::vector<unsigned char> download(const void* dev, size_t bytes, hipStr
 
 int main(int argc, char** argv) {
   if (argc < 6) {
-    printf("usage: %s model.onnx points.tensor xyz|zyx fp16|int8 output-prefix [aux]\n", argv[0]);
+    printf("usage: %s model.onnx points.tensor xyz|zyx fp16|int8|mxfp4 output-prefix [aux]\n", argv[0]);
     return 1;
   }
   hipStream_t stream;
@@ -58,7 +58,7 @@ int main(int argc, char** argv) {
   param.voxelization.max_points = (int)std::max(300000u, n_points);
   param.model = argv[1];
   param.order = !strcmp(argv[3], "zyx") ? CoordinateOrder::ZYX : CoordinateOrder::XYZ;
-  param.precision = !strcmp(argv[4], "int8") ? Precision::Int8 : Precision::Float16;
+  param.precision = !strcmp(argv[4], "int8") ? Precision::Int8 : !strcmp(argv[4], "mxfp4") ? Precision::MxFp4 : Precision::Float16;
   param.with_auxiliary_stream = argc > 6 && !strcmp(argv[6], "aux");
   const std::string prefix = argv[5];
 

@@ -23,7 +23,8 @@ import numpy as np
 from . import capi
 from .onnx_dialect import Graph, save as save_onnx
 
-PRECISION = {"fp16": capi.PRECISION_FP16, "float16": capi.PRECISION_FP16, "int8": capi.PRECISION_INT8}
+PRECISION = {"fp16": capi.PRECISION_FP16, "float16": capi.PRECISION_FP16, "int8": capi.PRECISION_INT8,
+             "mxfp4": capi.PRECISION_MXFP4}
 
 
 def _stream_ptr(stream) -> C.c_void_p:
@@ -142,6 +143,7 @@ class Engine:
                 a = n.attrs
                 pr = lambda key: capi.PRECISION_INT8 if a.get(key, "") == "int8" else capi.PRECISION_FP16  # noqa: E731
                 if n.op_type == "SparseConvolution":
+                    prec = capi.PRECISION_MXFP4 if a.get("precision", "") == "mxfp4" else pr("precision")
                     w = np.ascontiguousarray(graph.initializers[n.inputs[1]], np.float16)
                     bias = np.ascontiguousarray(graph.initializers[n.inputs[2]], np.float16)
                     wr = np.ascontiguousarray(a.get("weight_dynamic_ranges", []), np.float32)
@@ -153,7 +155,7 @@ class Engine:
                         capi.i3(*a.get("padding", [0, 0, 0])), capi.i3(*a.get("dilation", [1, 1, 1])),
                         float(a.get("input_dynamic_range", 0.0)), int(a.get("subm", 0)),
                         int(a.get("output_bound", 150000)), 10000, str(a.get("rulebook", "")).encode(),
-                        pr("precision"), pr("output_precision"), n.outputs[0].encode(), int(a.get("inverse", 0)))
+                        prec, pr("output_precision"), n.outputs[0].encode(), int(a.get("inverse", 0)))
                 elif n.op_type in ("Add", "QuantAdd"):
                     out = L.scn_builder_push_add(b, n.name.encode(), tmap[n.inputs[0]], tmap[n.inputs[1]],
                                                  float(a.get("input0_dynamic_range", 0.0)),
