@@ -382,39 +382,274 @@ __global__ __launch_bounds__(512) void k_mx_product_few(const ProductArgs p) {
   }
 }
 
-// Any number of rows: a wave owns 32 rows x 32 output channels, both operands straight from memory.
-__global__ __launch_bounds__(256) void k_mx_product_tile(const ProductArgs p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// Bias, ReLU, residual and store of 8 consecutive channels of one row (one 16-byte store in fp16, two in fp32; rows of any
+// alignment).
+__device__ __forceinline__ void product_store8(const ProductArgs& p, uint32_t i, uint32_t j, float (&y)[8]) {
+  if (j + 8 > p.n) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (j + q < p.n) product_store(p, i, j + q, y[q]);
+    return;
+  }
+  if (p.bias) {
+    if (p.bias_fp32) {
+      float b[8];
+      __builtin_memcpy(b, (const float*)p.bias + j, 32);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) y[q] += b[q];
+    } else {
+      _Float16 b[8];
+      __builtin_memcpy(b, (const _Float16*)p.bias + j, 16);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) y[q] += (float)b[q];
+    }
+  }
+  if (p.relu) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) y[q] = y[q] > 0.f ? y[q] : 0.f;
+  }
+  if (p.res) {
+    const size_t at = (size_t)i * p.res_ld + j;
+    if (p.res_fp32) {
+      float r[8];
+      __builtin_memcpy(r, (const float*)p.res + at, 32);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) y[q] += r[q];
+    } else {
+      _Float16 r[8];
+      __builtin_memcpy(r, (const _Float16*)p.res + at, 16);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) y[q] += (float)r[q];
+    }
+  }
+  if (p.relu2) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) y[q] = y[q] > 0.f ? y[q] : 0.f;
+  }
+  const size_t at = (size_t)i * p.out_ld + j;
+  if (p.out_fp32) {
+    __builtin_memcpy((float*)p.out + at, y, 32);
+  } else {
+    _Float16 h[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) h[q] = (_Float16)y[q];
+    __builtin_memcpy((_Float16*)p.out + at, h, 16);
+  }
+}
+
+// Any number of rows.  A workgroup of 4 * WN * WM... waves owns BN output channels x BM rows; both operands are staged
+// through LDS, 256 channels (8 blocks = 128 code bytes and 8 scale bytes per row) at a time, by loads that go straight to
+// LDS, two stages deep.
+//   LDS of a stage: codes of the BN weight rows, codes of the BM rows (128 bytes each), then their scales (8 bytes each).
+//   Block c of row r lies at position c ^ (r / 2) % 8 of its row, so that the 16-byte operand reads of 16 neighbouring rows
+//   touch all 64 banks once (rows of 128 bytes: two rows fill the banks).  The hardware places lane l's bytes at base + 16 l,
+//   so the order is obtained by permuting which block a lane fetches.
+//   A wave owns TN x TM tiles of 32 x 32: per matrix instruction of 64 channels it reads (TN + TM) KB from LDS for TN * TM
+//   products.
+// Rows beyond the last are read as the last one and not stored; blocks beyond the last come from a page of zeros.
+__device__ uint4 g_mx_zero[1];   // (device globals are zeroed)
+
+typedef const __attribute__((address_space(1))) void* mx_gptr;
+typedef __attribute__((address_space(3))) void* mx_lptr;
+
+template <int TN, int TM>
+__device__ __forceinline__ void mx_read_operands(uint32_t addr, v4i (&w)[TN], v4i (&x)[TM], uint32_t x_addr) {
+  // one block with its own wait: the outputs are complete when it ends
+  if constexpr (TN == 4 && TM == 2)
+    asm volatile("ds_read_b128 %0, %6\n\tds_read_b128 %4, %7\n\tds_read_b128 %1, %6 offset:4096\n\tds_read_b128 %5, %7 offset:4096\n\t"
+                 "ds_read_b128 %2, %6 offset:8192\n\tds_read_b128 %3, %6 offset:12288\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(x[0]), "=&v"(x[1])
+                 : "v"(addr), "v"(x_addr)
+                 : "memory");
+  else if constexpr (TN == 2 && TM == 2)
+    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %2, %5\n\tds_read_b128 %1, %4 offset:4096\n\tds_read_b128 %3, %5 offset:4096\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(w[0]), "=&v"(w[1]), "=&v"(x[0]), "=&v"(x[1])
+                 : "v"(addr), "v"(x_addr)
+                 : "memory");
+  else
+    asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(w[0]), "=&v"(x[0])
+                 : "v"(addr), "v"(x_addr)
+                 : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void mx_read_scales(uint32_t addr, uint2 (&s)[N]) {
+  uint64_t t[N];
+  if constexpr (N == 4)
+    asm volatile("ds_read_b64 %0, %4\n\tds_read_b64 %1, %4 offset:256\n\tds_read_b64 %2, %4 offset:512\n\tds_read_b64 %3, %4 offset:768\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(t[0]), "=&v"(t[1]), "=&v"(t[2]), "=&v"(t[3])
+                 : "v"(addr)
+                 : "memory");
+  else if constexpr (N == 2)
+    asm volatile("ds_read_b64 %0, %2\n\tds_read_b64 %1, %2 offset:256\n\ts_waitcnt lgkmcnt(0)" : "=&v"(t[0]), "=&v"(t[1]) : "v"(addr) : "memory");
+  else
+    asm volatile("ds_read_b64 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(t[0]) : "v"(addr) : "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) s[i] = make_uint2((uint32_t)t[i], (uint32_t)(t[i] >> 32));
+}
+
+// (the byte of the scale registers is an immediate of the instruction)
+template <int SEL>
+__device__ __forceinline__ v16f mx_mma32_sel(const v4i& a, uint32_t sa, const v4i& b, uint32_t sb, v16f c) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v8i{a[0], a[1], a[2], a[3], 0, 0, 0, 0}, v8i{b[0], b[1], b[2], b[3], 0, 0, 0, 0},
+                                                         c, 4, 4, SEL, (int)sa, SEL, (int)sb);
+}
+
+template <int BN, int BM, int TN, int TM>
+struct ProductTile {
+  static constexpr int WN = BN / (32 * TN), WM = BM / (32 * TM), WAVES = WN * WM;
+  static constexpr int STAGE = (BN + BM) * 136;                       // bytes of LDS per stage
+  static constexpr int PAD = 32 * TN + 4;                             // floats per row of the store buffer
+  static constexpr int STORE = WAVES * 32 * PAD * 4;
+  static size_t lds(uint32_t stages) { return std::max<size_t>((stages > 1 ? 2 : 1) * (size_t)STAGE, STORE); }
+};
+
+template <int BN, int BM, int TN, int TM>
+constexpr int kProductThreads = 64 * ProductTile<BN, BM, TN, TM>::WAVES;
+
+template <int BN, int BM, int TN, int TM>
+__global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_product_lds(const ProductArgs p, uint32_t tiles_n,
+                                                                                              uint32_t tiles_m) {
+  using T = ProductTile<BN, BM, TN, TM>;
+  constexpr int WAVES = T::WAVES, STAGE = T::STAGE;
+  constexpr int CODE_LOADS = (BN + BM) / 8 / WAVES, SCALE_LOADS = (BN + BM) / 32 / WAVES;   // wave loads per stage
+  static_assert(CODE_LOADS * 8 * WAVES == BN + BM && SCALE_LOADS * 32 * WAVES == BN + BM, "loads do not divide");
+  extern __shared__ __align__(16) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, lh = lane >> 5;
   const uint32_t m = eff_n(p.m_dev, p.m);
-  const uint32_t i0 = blockIdx.x * 32, n0 = (blockIdx.y * 4 + wave) * 32;
-  if (i0 >= m || n0 >= p.n) return;
-  const uint32_t brow = min(n0 + ln, p.n - 1), arow = min(i0 + ln, m - 1);
-  const uint8_t* bc = p.b + (size_t)brow * p.b_ld;
-  const uint8_t* bsc = p.bs + (size_t)brow * p.bs_ld;
-  const uint8_t* ac = (const uint8_t*)p.a + (size_t)arow * p.a_ld;
-  const uint8_t* asc = p.as + (size_t)arow * p.as_ld;
-  v16f acc;
+  // XCD x takes the x-th contiguous eighth of the tiles (each XCD has its own L2), in bands of 8 row tiles that are walked
+  // channel tile by channel tile, so that the tiles in flight on an XCD form a rectangle and share operands
+  const uint32_t total = tiles_n * tiles_m, per = (total + 7) / 8;
+  const uint32_t t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= per || t >= total) return;
+  const uint32_t band = t / (8 * tiles_n), in_band = t - band * 8 * tiles_n;
+  const uint32_t rows_in_band = min(8u, tiles_m - band * 8);
+  const uint32_t tm = band * 8 + in_band % rows_in_band, tn = in_band / rows_in_band;
+  const uint32_t i0 = tm * BM, n0 = tn * BN;
+  if (i0 >= m) return;
+
+  // what this lane fetches: code load q covers 8 rows (lane / 8), position lane % 8; scale load q 32 rows (lane / 2)
+  const uint8_t* csrc[CODE_LOADS];
+  const uint8_t* ssrc[SCALE_LOADS];
+  const uint8_t* zero = reinterpret_cast<const uint8_t*>(g_mx_zero);
+  uint32_t cblk;   // block of a stage this lane fetches (the same for every load: rows advance by multiples of 16)
+  {
+    static_assert(WAVES % 2 == 0, "rows of one lane differ by multiples of 16");
+    const int r0 = wave * 8 + (lane >> 3);
+    cblk = (lane & 7) ^ ((r0 >> 1) & 7);
 #pragma unroll
-  for (int j = 0; j < 16; ++j) acc[j] = 0.f;
-  for (uint32_t s = 0; s < (p.kb + 1) / 2; ++s) {
-    const uint32_t blk = 2 * s + lh;
-    uint4 wq = make_uint4(0, 0, 0, 0), xq = make_uint4(0, 0, 0, 0);
-    int ws = 0, xs = 0;
-    if (blk < p.kb) {
-      wq = *reinterpret_cast<const uint4*>(bc + (size_t)blk * 16);
-      xq = *reinterpret_cast<const uint4*>(ac + (size_t)blk * 16);
-      ws = bsc[blk];
-      xs = asc[blk];
+    for (int q = 0; q < CODE_LOADS; ++q) {
+      const uint32_t r = q * WAVES * 8 + r0;   // BN is a multiple of WAVES * 8: a load is all weights or all rows
+      const bool is_w = q * WAVES * 8 < BN;
+      const size_t row = is_w ? min(n0 + r, p.n - 1) : min(i0 + r - BN, m - 1);
+      csrc[q] = (is_w ? p.b + row * p.b_ld : (const uint8_t*)p.a + row * p.a_ld) + cblk * 16;
     }
-    acc = mx_mma32(wq, ws, xq, xs, acc);
-  }
-  if (i0 + ln >= m) return;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const uint32_t ch = n0 + 8 * (j / 4) + 4 * lh + j % 4;
-    if (ch < p.n) product_store(p, i0 + ln, ch, acc[j]);
+    for (int q = 0; q < SCALE_LOADS; ++q) {
+      const uint32_t r = q * WAVES * 32 + wave * 32 + (lane >> 1);
+      const bool is_w = r < BN;
+      const size_t row = is_w ? min(n0 + r, p.n - 1) : min(i0 + r - BN, m - 1);
+      ssrc[q] = (is_w ? p.bs + row * p.bs_ld : p.as + row * p.as_ld) + (lane & 1) * 4;
+    }
   }
+  const uint32_t stages = (p.kb + 7) / 8;
+  auto load = [&](uint32_t st) {
+    char* buf = lds + (st & 1) * STAGE;
+    const bool in = st * 8 + cblk < p.kb;
+#pragma unroll
+    for (int q = 0; q < CODE_LOADS; ++q)
+      __builtin_amdgcn_global_load_lds((mx_gptr)(in ? csrc[q] + (size_t)st * 128 : zero), (mx_lptr)(buf + (q * WAVES + wave) * 1024), 16, 0, 0);
+    const bool sin = st * 8 + (lane & 1) * 4 < p.kb;
+#pragma unroll
+    for (int q = 0; q < SCALE_LOADS; ++q)
+      __builtin_amdgcn_global_load_lds((mx_gptr)(sin ? ssrc[q] + (size_t)st * 8 : zero),
+                                       (mx_lptr)(buf + (BN + BM) * 128 + (q * WAVES + wave) * 256), 4, 0, 0);
+  };
+
+  v16f acc[TN][TM];
+#pragma unroll
+  for (int a = 0; a < TN; ++a)
+#pragma unroll
+    for (int b = 0; b < TM; ++b)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[a][b][j] = 0.f;
+
+  const int wn = wave % T::WN, wm = wave / T::WN;
+  const uint32_t base = (uint32_t)(uintptr_t)(mx_lptr)lds;
+  const uint32_t w_row = wn * 32 * TN + ln, x_row = BN + wm * 32 * TM + ln;
+  const uint32_t swz = (ln >> 1) & 7;
+  load(0);
+  for (uint32_t st = 0; st < stages; ++st) {
+    if (st + 1 < stages) {
+      load(st + 1);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CODE_LOADS + SCALE_LOADS) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    __builtin_amdgcn_s_barrier();
+    const uint32_t sb = base + (st & 1) * STAGE;
+    const uint32_t left = p.kb - st * 8;   // blocks from here on
+    const uint32_t mask0 = left >= 4 ? ~0u : (1u << (8 * left)) - 1u;
+    const uint32_t mask1 = left >= 8 ? ~0u : left > 4 ? (1u << (8 * (left - 4))) - 1u : 0u;
+    uint2 ws[TN], xs[TM];
+    mx_read_scales<TN>(sb + (BN + BM) * 128 + w_row * 8, ws);
+    mx_read_scales<TM>(sb + (BN + BM) * 128 + x_row * 8, xs);
+    // blocks 2 s + lh of step s: bytes 0 and 2 of the two words after a shift by lh bytes
+#pragma unroll
+    for (int a = 0; a < TN; ++a) ws[a] = make_uint2((ws[a].x & mask0) >> (8 * lh), (ws[a].y & mask1) >> (8 * lh));
+#pragma unroll
+    for (int b = 0; b < TM; ++b) xs[b] = make_uint2((xs[b].x & mask0) >> (8 * lh), (xs[b].y & mask1) >> (8 * lh));
+#define SCN_MX_STEP(S, SEL, WORD)                                                                  \
+  if (2 * (S) < left) {                                                                            \
+    v4i w[TN], x[TM];                                                                              \
+    const uint32_t pos = ((2 * (S) + lh) ^ swz) * 16;                                              \
+    mx_read_operands<TN, TM>(sb + w_row * 128 + pos, w, x, sb + x_row * 128 + pos);                \
+    _Pragma("unroll") for (int a = 0; a < TN; ++a) _Pragma("unroll") for (int b = 0; b < TM; ++b)  \
+        acc[a][b] = mx_mma32_sel<SEL>(w[a], ws[a].WORD, x[b], xs[b].WORD, acc[a][b]);              \
+  }
+    SCN_MX_STEP(0, 0, x)
+    SCN_MX_STEP(1, 2, x)
+    SCN_MX_STEP(2, 0, y)
+    SCN_MX_STEP(3, 2, y)
+#undef SCN_MX_STEP
+    __builtin_amdgcn_s_barrier();
+  }
+  // Store through LDS (wave-private, 32 rows at a time): a lane of the accumulators holds 4 consecutive channels of one
+  // row, a store wants whole 128-byte lines of a row.
+  float* buf = reinterpret_cast<float*>(lds) + wave * 32 * T::PAD;
+  constexpr int LPR = 4 * TN, RPP = 64 / LPR;   // lanes per row (8 channels each), rows per pass
+#pragma unroll
+  for (int b = 0; b < TM; ++b) {
+#pragma unroll
+    for (int a = 0; a < TN; ++a)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<v4f*>(buf + ln * T::PAD + a * 32 + q * 8 + lh * 4) =
+            v4f{acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]};
+    const uint32_t row0 = i0 + wm * 32 * TM + b * 32, ch = n0 + wn * 32 * TN + (lane % LPR) * 8;
+#pragma unroll 2
+    for (int r = lane / LPR; r < 32; r += RPP) {
+      float y[8];
+      *reinterpret_cast<v4f*>(y) = *reinterpret_cast<const v4f*>(buf + r * T::PAD + (lane % LPR) * 8);
+      *reinterpret_cast<v4f*>(y + 4) = *reinterpret_cast<const v4f*>(buf + r * T::PAD + (lane % LPR) * 8 + 4);
+      if (row0 + r < m && ch < p.n) product_store8(p, row0 + r, ch, y);
+    }
+  }
+}
+
+template <int BN, int BM, int TN, int TM>
+static int launch_product(const ProductArgs& p, hipStream_t stream) {
+  using T = ProductTile<BN, BM, TN, TM>;
+  const uint64_t tn = ((uint64_t)p.n + BN - 1) / BN, tm = ((uint64_t)p.m + BM - 1) / BM;
+  SCN_REQUIRE(tn * tm < (1ull << 27), SCN_ERR_UNSUPPORTED, "mx_product: %u x %u outputs are too many for one call", p.m, p.n);
+  const size_t lds = T::lds((p.kb + 7) / 8);
+  hipLaunchKernelGGL((k_mx_product_lds<BN, BM, TN, TM>), dim3((unsigned)((tn * tm + 7) / 8 * 8)), dim3(64 * T::WAVES), lds, stream, p,
+                     (uint32_t)tn, (uint32_t)tm);
+  return SCN_OK;
 }
 
 constexpr uint32_t kDirectRows = 16;
@@ -490,8 +725,12 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
     else if (at == SCN_DTYPE_FP16) hipLaunchKernelGGL(k_mx_product_few<SCN_DTYPE_FP16>, grid, dim3(512), 0, stream, p);
     else hipLaunchKernelGGL(k_mx_product_few<SCN_DTYPE_FP32>, grid, dim3(512), 0, stream, p);
   } else {
-    SCN_REQUIRE(ceil_div(io.n, 128) <= 65535u, SCN_ERR_UNSUPPORTED, "mx_product: n = %u is too large", io.n);
-    hipLaunchKernelGGL(k_mx_product_tile, dim3(ceil_div(io.m, 32), ceil_div(io.n, 128)), dim3(256), 0, stream, p);
+    // the largest tile of which there are enough for the GPU's 256 CUs
+    const uint64_t t256 = (uint64_t)ceil_div(io.n, 256) * ceil_div(io.m, 256), t128 = (uint64_t)ceil_div(io.n, 128) * ceil_div(io.m, 128);
+    int rc = t256 >= 256 && kb > 8 ? launch_product<256, 256, 4, 2>(p, stream)
+             : t128 >= 256         ? launch_product<128, 128, 2, 2>(p, stream)
+                                   : launch_product<64, 64, 1, 1>(p, stream);
+    if (rc) return rc;
   }
   SCN_HIP(hipGetLastError());
   return SCN_OK;

@@ -10,7 +10,9 @@ rows" in scn_c_api.h for the format).  PyTorch only owns memory and streams; the
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
+import struct
 from typing import Optional, Sequence
 
 import numpy as np
@@ -20,6 +22,30 @@ from . import capi
 from .scn import _stream_ptr
 
 _DTYPE = {torch.float16: capi.DTYPE_FP16, torch.float32: capi.DTYPE_FP32, torch.int8: capi.DTYPE_INT8}
+_FLOATS = (torch.float16, torch.float32)
+_HERE = contextlib.nullcontext()
+_L = None
+
+
+def _lib():
+    global _L
+    if _L is None:
+        _L = capi.lib()
+    return _L
+
+
+def _on(index: int):
+    """The rows' device as the current one (these calls take a few microseconds: no context is entered without need)."""
+    return _HERE if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # (a tenth of the time of building a Stream object)
+
+
+def _stream(stream, index: int):
+    if stream is not None:
+        return _stream_ptr(stream)
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 def row_bytes(channels: int) -> int:
@@ -31,93 +57,130 @@ def row_bytes(channels: int) -> int:
 class MxRows:
     """codes [n, >= 16 * blocks] and scales [n, >= round_up(blocks, 4)] (uint8, unit stride inside a row) of n rows."""
 
+    __slots__ = ("_codes", "_scales", "_buffer", "channels", "num_rows", "index", "codes_ptr", "codes_ld", "scales_ptr", "scales_ld")
+
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, channels: int):
-        for t, need in ((codes, 16 * ((channels + 31) // 32)), (scales, ((channels + 31) // 32 + 3) // 4 * 4)):
+        if channels < 1:
+            raise ValueError("rows need at least one channel")
+        blocks = (channels + 31) // 32
+        for t, need in ((codes, 16 * blocks), (scales, (blocks + 3) // 4 * 4)):
             if t.dtype != torch.uint8 or t.dim() != 2 or not t.is_cuda:
                 raise ValueError("codes and scales must be 2-D uint8 device tensors")
-            if t.shape[1] < need or (t.shape[1] > 1 and t.stride(1) != 1):
-                raise ValueError(f"rows of {channels} channels need {need} contiguous bytes")
+            if t.shape[1] < need or t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < need):
+                raise ValueError(f"rows of {channels} channels need {need} contiguous bytes of their own")
         if codes.shape[0] != scales.shape[0] or codes.device != scales.device:
             raise ValueError("codes and scales must have the same rows on the same device")
-        self.codes, self.scales, self.channels = codes, scales, int(channels)
-
-    @property
-    def num_rows(self) -> int:
-        return int(self.codes.shape[0])
-
-    @property
-    def device(self):
-        return self.codes.device
+        self._codes, self._scales, self._buffer = codes, scales, None
+        self.channels, self.num_rows, self.index = int(channels), int(codes.shape[0]), codes.get_device()
+        self.codes_ptr, self.codes_ld = codes.data_ptr(), _ld(codes)
+        self.scales_ptr, self.scales_ld = scales.data_ptr(), _ld(scales)
 
     @classmethod
     def empty(cls, n: int, channels: int, device="cuda") -> "MxRows":
         """Uninitialised rows in the one-buffer form."""
         if channels < 1 or n < 0:
             raise ValueError("rows need at least one channel")
-        blocks = (channels + 31) // 32
-        buf = torch.empty((n, row_bytes(channels)), dtype=torch.uint8, device=device)
-        return cls(buf[:, :16 * blocks], buf[:, 16 * blocks:16 * blocks + (blocks + 3) // 4 * 4], channels)
+        self = cls.__new__(cls)
+        size = row_bytes(channels)
+        buf = torch.empty((n, size), dtype=torch.uint8, device=device)
+        self._codes = self._scales = None
+        self._buffer, self.channels, self.num_rows, self.index = buf, int(channels), int(n), buf.get_device()
+        self.codes_ptr = buf.data_ptr()
+        self.scales_ptr = self.codes_ptr + 16 * ((channels + 31) // 32)
+        self.codes_ld = self.scales_ld = size
+        return self
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._codes = self._buffer[:, :16 * ((self.channels + 31) // 32)]
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            blocks = (self.channels + 31) // 32
+            self._scales = self._buffer[:, 16 * blocks:16 * blocks + (blocks + 3) // 4 * 4]
+        return self._scales
+
+    @property
+    def device(self) -> torch.device:
+        return torch.device("cuda", self.index)
 
 
-def _check_rows(x: torch.Tensor, dtypes, what: str) -> None:
+def _check_rows(x: torch.Tensor, dtypes, what: str) -> int:
+    """Refuses what is not rows of a device tensor; returns the row stride in elements."""
     if not isinstance(x, torch.Tensor) or x.dtype not in dtypes or x.dim() != 2 or not x.is_cuda:
         raise ValueError(f"{what} must be a 2-D device tensor of {' or '.join(str(d) for d in dtypes)}")
-    if x.shape[1] > 1 and x.stride(1) != 1:
+    n, c = x.shape
+    ld, step = x.stride()
+    if c > 1 and step != 1:
         raise ValueError(f"{what} must have unit stride inside a row")
-    if x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+    if n > 1 and ld < c:
         raise ValueError(f"{what} must not have overlapping rows")
+    return ld if n > 1 else max(ld, c)
 
 
 def _ld(x: torch.Tensor) -> int:
     return int(x.stride(0)) if x.shape[0] > 1 else max(int(x.stride(0)), int(x.shape[1]))
 
 
-def _count_ptr(num: Optional[torch.Tensor], device) -> Optional[int]:
+def _count_ptr(num: Optional[torch.Tensor], index: int) -> Optional[int]:
     if num is None:
         return None
-    if num.dtype not in (torch.int32, torch.uint32) or num.numel() != 1 or num.device != device:
+    if num.dtype not in (torch.int32, torch.uint32) or num.numel() != 1 or not num.is_cuda or num.get_device() != index:
         raise ValueError("num must be one int32 / uint32 on the rows' device")
     return num.data_ptr()
 
 
-def _same_device(device, *others) -> None:
+def _same_device(index: int, *others) -> None:
     for t in others:
-        if t is not None and t.device != device:
-            raise ValueError(f"tensors on {device} and {t.device}")
+        if t is not None and (t.index if isinstance(t, MxRows) else t.get_device()) != index:
+            raise ValueError(f"tensors on different devices (rows on cuda:{index})")
 
 
 def quantize_rows(x: torch.Tensor, relu: bool = False, dynamic_range: float = 0.0, num: Optional[torch.Tensor] = None,
                   out: Optional[MxRows] = None, stream=None) -> MxRows:
     """x: fp16, fp32 or int8 (value = q * dynamic_range / 127) rows [n, c]; num: device-side row count (rows beyond it are
     left as they were)."""
-    _check_rows(x, (torch.float16, torch.float32, torch.int8), "x")
+    ld = _check_rows(x, (torch.float16, torch.float32, torch.int8), "x")
     n, c = x.shape
-    if out is None:
-        out = MxRows.empty(n, c, x.device)
-    elif out.num_rows < n or out.channels != c:
-        raise ValueError("out does not fit x")
-    _same_device(x.device, out)
-    with torch.cuda.device(x.device):
-        capi.check(capi.lib().scn_mx_quantize_rows(
-            x.data_ptr(), _DTYPE[x.dtype], c, _ld(x), float(dynamic_range), int(bool(relu)), out.codes.data_ptr(), _ld(out.codes),
-            out.scales.data_ptr(), _ld(out.scales), n, _count_ptr(num, x.device), _stream_ptr(stream)))
+    index = x.get_device()
+    with _on(index):
+        if out is None:
+            out = MxRows.empty(n, c, x.device)
+        elif out.num_rows < n or out.channels != c or out.index != index:
+            raise ValueError("out does not fit x")
+        rc = _lib().scn_mx_quantize_rows(x.data_ptr(), _DTYPE[x.dtype], c, ld, dynamic_range, relu, out.codes_ptr, out.codes_ld,
+                                         out.scales_ptr, out.scales_ld, n, _count_ptr(num, index), _stream(stream, index))
+    if rc:
+        capi.check(rc)
     return out
 
 
 def dequantize_rows(rows: MxRows, dtype: torch.dtype = torch.float16, num: Optional[torch.Tensor] = None,
                     out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
-    n, c = rows.num_rows, rows.channels
-    if out is None:
-        out = torch.empty((n, c), dtype=dtype, device=rows.device)
-    _check_rows(out, (torch.float16, torch.float32), "out")
-    if out.shape[0] < n or out.shape[1] != c:
-        raise ValueError("out does not fit the rows")
-    _same_device(rows.device, out)
-    with torch.cuda.device(rows.device):
-        capi.check(capi.lib().scn_mx_dequantize_rows(
-            rows.codes.data_ptr(), _ld(rows.codes), rows.scales.data_ptr(), _ld(rows.scales), c, out.data_ptr(),
-            _DTYPE[out.dtype], _ld(out), n, _count_ptr(num, rows.device), _stream_ptr(stream)))
+    n, c, index = rows.num_rows, rows.channels, rows.index
+    with _on(index):
+        if out is None:
+            if dtype not in _FLOATS:
+                raise ValueError("dtype must be float16 or float32")
+            out, ld = torch.empty((n, c), dtype=dtype, device="cuda"), c
+        else:
+            ld = _check_rows(out, _FLOATS, "out")
+            if out.shape[0] < n or out.shape[1] != c:
+                raise ValueError("out does not fit the rows")
+            _same_device(index, out)
+        rc = _lib().scn_mx_dequantize_rows(rows.codes_ptr, rows.codes_ld, rows.scales_ptr, rows.scales_ld, c, out.data_ptr(),
+                                           _DTYPE[out.dtype], ld, n, _count_ptr(num, index), _stream(stream, index))
+    if rc:
+        capi.check(rc)
     return out
+
+
+# scn_mx_product_io as native bytes (same layout as capi.MxProductIO, filled in one go)
+_PRODUCT_IO = struct.Struct("PiIPIPIPIIIIPPiiPiIiPiIPN")
+assert _PRODUCT_IO.size == C.sizeof(capi.MxProductIO)
 
 
 def product(a, b: MxRows, bias: Optional[torch.Tensor] = None, relu: bool = False, residual: Optional[torch.Tensor] = None,
@@ -126,50 +189,57 @@ def product(a, b: MxRows, bias: Optional[torch.Tensor] = None, relu: bool = Fals
     """relu2(relu(a b^T + bias) + residual): a is MxRows, or fp16 / fp32 rows that are quantised on the way; b the rows of a
     weight matrix.  workspace: uint8 scratch for the quantised rows (a new one is allocated when it is needed and not
     given); calls that may overlap need one each."""
-    L = capi.lib()
-    io = capi.MxProductIO()
-    if isinstance(a, MxRows):
-        m, k = a.num_rows, a.channels
-        io.a_dev, io.a_dtype, io.a_ld = a.codes.data_ptr(), capi.DTYPE_MXFP4, _ld(a.codes)
-        io.a_scales_dev, io.a_scales_ld = a.scales.data_ptr(), _ld(a.scales)
-    else:
-        _check_rows(a, (torch.float16, torch.float32), "a")
-        m, k = a.shape
-        io.a_dev, io.a_dtype, io.a_ld = a.data_ptr(), _DTYPE[a.dtype], _ld(a)
-    n = b.num_rows
-    if b.channels != k:
-        raise ValueError(f"rows of {k} channels times weights of {b.channels}")
-    device = b.device
-    if out is None:
-        out = torch.empty((m, n), dtype=out_dtype, device=device)
-    _check_rows(out, (torch.float16, torch.float32), "out")
-    if out.shape[0] < m or out.shape[1] != n:
-        raise ValueError("out does not fit the product")
-    if bias is not None and (bias.dtype not in (torch.float16, torch.float32) or bias.shape != (n,) or not bias.is_contiguous()):
-        raise ValueError(f"bias must be {n} contiguous fp16 or fp32 values")
-    if residual is not None:
-        _check_rows(residual, (torch.float16, torch.float32), "residual")
-        if residual.shape[0] < m or residual.shape[1] != n:
-            raise ValueError("residual does not fit the product")
-    _same_device(device, a, out, bias, residual, workspace)
-    with torch.cuda.device(device):
-        if not isinstance(a, MxRows):
-            need = int(L.scn_mx_product_workspace(m, k))
-            if need and workspace is None:
-                workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    L = _lib()
+    n, index = b.num_rows, b.index
+    with _on(index):
+        ws_ptr = ws_bytes = 0
+        if isinstance(a, MxRows):
+            m, k, a_index = a.num_rows, a.channels, a.index
+            a_ptr, a_dtype, a_ld, as_ptr, as_ld = a.codes_ptr, capi.DTYPE_MXFP4, a.codes_ld, a.scales_ptr, a.scales_ld
+        else:
+            a_ld = _check_rows(a, _FLOATS, "a")
+            (m, k), a_index = a.shape, a.get_device()
+            a_ptr, a_dtype, as_ptr, as_ld = a.data_ptr(), _DTYPE[a.dtype], 0, 0
+            if workspace is None:
+                ws_bytes = L.scn_mx_product_workspace(m, k)
+                if ws_bytes:
+                    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device="cuda")
             if workspace is not None:
-                io.workspace_dev, io.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        io.b_codes_dev, io.b_codes_ld = b.codes.data_ptr(), _ld(b.codes)
-        io.b_scales_dev, io.b_scales_ld = b.scales.data_ptr(), _ld(b.scales)
-        io.m, io.n, io.k = m, n, k
-        io.m_dev = _count_ptr(num, device)
+                if not workspace.is_contiguous():
+                    raise ValueError("workspace must be contiguous")
+                _same_device(index, workspace)
+                ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        if a_index != index:
+            raise ValueError(f"rows on cuda:{a_index}, weights on cuda:{index}")
+        if b.channels != k:
+            raise ValueError(f"rows of {k} channels times weights of {b.channels}")
+        if out is None:
+            if out_dtype not in _FLOATS:
+                raise ValueError("out_dtype must be float16 or float32")
+            out, out_ld = torch.empty((m, n), dtype=out_dtype, device="cuda"), n
+        else:
+            out_ld = _check_rows(out, _FLOATS, "out")
+            if out.shape[0] < m or out.shape[1] != n:
+                raise ValueError("out does not fit the product")
+            _same_device(index, out)
+        bias_ptr = bias_dtype = res_ptr = res_dtype = res_ld = 0
         if bias is not None:
-            io.bias_dev, io.bias_dtype = bias.data_ptr(), _DTYPE[bias.dtype]
-        io.relu, io.relu_after_add = int(bool(relu)), int(bool(relu_after_add))
+            if bias.dtype not in _FLOATS or bias.shape != (n,) or not bias.is_contiguous():
+                raise ValueError(f"bias must be {n} contiguous fp16 or fp32 values")
+            _same_device(index, bias)
+            bias_ptr, bias_dtype = bias.data_ptr(), _DTYPE[bias.dtype]
         if residual is not None:
-            io.res_dev, io.res_dtype, io.res_ld = residual.data_ptr(), _DTYPE[residual.dtype], _ld(residual)
-        io.out_dev, io.out_dtype, io.out_ld = out.data_ptr(), _DTYPE[out.dtype], _ld(out)
-        capi.check(L.scn_mx_product(C.byref(io), _stream_ptr(stream)))
+            res_ld = _check_rows(residual, _FLOATS, "residual")
+            if residual.shape[0] < m or residual.shape[1] != n:
+                raise ValueError("residual does not fit the product")
+            _same_device(index, residual)
+            res_ptr, res_dtype = residual.data_ptr(), _DTYPE[residual.dtype]
+        rc = L.scn_mx_product(_PRODUCT_IO.pack(a_ptr, a_dtype, a_ld, as_ptr, as_ld, b.codes_ptr, b.codes_ld, b.scales_ptr, b.scales_ld,
+                                               m, n, k, _count_ptr(num, index) or 0, bias_ptr, bias_dtype, bool(relu), res_ptr,
+                                               res_dtype, res_ld, bool(relu_after_add), out.data_ptr(), _DTYPE[out.dtype], out_ld,
+                                               ws_ptr, ws_bytes), _stream(stream, index))
+    if rc:
+        capi.check(rc)
     return out
 
 
@@ -192,7 +262,7 @@ class Rulebook:
         self._check(indices)
         self._keep = (indices, num)
         capi.check(capi.lib().scn_rulebook_build_subm(
-            self._h, indices.data_ptr(), int(indices.shape[0]), _count_ptr(num, indices.device), capi.i3(*grid),
+            self._h, indices.data_ptr(), int(indices.shape[0]), _count_ptr(num, indices.get_device()), capi.i3(*grid),
             capi.i3(*kernel_size), capi.i3(*dilation), _stream_ptr(stream)))
         self.rows_in = self.rows_out = min(int(indices.shape[0]), self.max_in)
 
@@ -201,7 +271,7 @@ class Rulebook:
         self._check(indices)
         self._keep = (indices, num)
         capi.check(capi.lib().scn_rulebook_build_sparse(
-            self._h, indices.data_ptr(), int(indices.shape[0]), _count_ptr(num, indices.device), capi.i3(*grid),
+            self._h, indices.data_ptr(), int(indices.shape[0]), _count_ptr(num, indices.get_device()), capi.i3(*grid),
             capi.i3(*kernel_size), capi.i3(*stride), capi.i3(*padding), capi.i3(*dilation), _stream_ptr(stream)))
         self.rows_in, self.rows_out = min(int(indices.shape[0]), self.max_in), self.max_out
 
@@ -211,7 +281,8 @@ class Rulebook:
             self._h = None
 
     def __del__(self):
-        self.close()
+        if capi is not None:      # (None while the interpreter ends)
+            self.close()
 
 
 class Conv:
@@ -242,26 +313,30 @@ class Conv:
             raise ValueError(f"the rulebook covers {rulebook.rows_in} input rows and up to {rulebook.rows_out} output rows")
         if x.channels != self.cin:
             raise ValueError(f"input rows have {x.channels} channels, the weight expects {self.cin}")
-        if _ld(x.codes) != _ld(x.scales) or x.scales.data_ptr() != x.codes.data_ptr() + 16 * blocks:
+        if x.codes_ld != x.scales_ld or x.scales_ptr != x.codes_ptr + 16 * blocks:
             raise ValueError("the convolution reads rows in the one-buffer form (codes, then scales)")
         wide = (self.cout + 15) // 16 * 16
-        if out is None:
-            out = torch.empty((max_rows, wide), dtype=torch.float16, device=x.device)
-        _check_rows(out, (torch.float16,), "out")
-        if out.shape[0] < max_rows or out.shape[1] < wide:
-            raise ValueError(f"out must hold {max_rows} rows of {wide} channels")
-        _same_device(x.device, out, residual)
-        io = capi.ConvIO()
-        io.x_dev, io.x_ld = x.codes.data_ptr(), _ld(x.codes)
-        io.relu, io.out_dtype, io.out_dev, io.out_ld = int(bool(relu)), capi.DTYPE_FP16, out.data_ptr(), _ld(out)
-        if residual is not None:
-            _check_rows(residual, (torch.float16,), "residual")
-            if residual.shape[0] < max_rows or residual.shape[1] < wide:
-                raise ValueError(f"residual must hold {max_rows} rows of {wide} channels")
-            io.res_dev, io.res_dtype, io.res_ld, io.mid_dtype = residual.data_ptr(), capi.DTYPE_FP16, _ld(residual), capi.DTYPE_FP16
-            io.relu_after_add = int(bool(relu_after_add))
-        with torch.cuda.device(x.device):
-            capi.check(capi.lib().scn_conv_forward(self._h, rulebook._h, C.byref(io), _stream_ptr(stream)))
+        with _on(x.index):
+            if out is None:
+                out, out_ld = torch.empty((max_rows, wide), dtype=torch.float16, device="cuda"), wide
+            else:
+                out_ld = _check_rows(out, (torch.float16,), "out")
+                if out.shape[0] < max_rows or out.shape[1] < wide:
+                    raise ValueError(f"out must hold {max_rows} rows of {wide} channels")
+                _same_device(x.index, out)
+            io = capi.ConvIO()
+            io.x_dev, io.x_ld = x.codes_ptr, x.codes_ld
+            io.relu, io.out_dtype, io.out_dev, io.out_ld = int(bool(relu)), capi.DTYPE_FP16, out.data_ptr(), out_ld
+            if residual is not None:
+                io.res_ld = _check_rows(residual, (torch.float16,), "residual")
+                if residual.shape[0] < max_rows or residual.shape[1] < wide:
+                    raise ValueError(f"residual must hold {max_rows} rows of {wide} channels")
+                _same_device(x.index, residual)
+                io.res_dev, io.res_dtype, io.mid_dtype = residual.data_ptr(), capi.DTYPE_FP16, capi.DTYPE_FP16
+                io.relu_after_add = int(bool(relu_after_add))
+            capi.check(_lib().scn_conv_forward(self._h, rulebook._h, C.byref(io), _stream(stream, x.index)))
+        if out.shape == (max_rows, self.cout):
+            return out
         return out[:max_rows, :self.cout]
 
     def close(self):
@@ -270,4 +345,5 @@ class Conv:
             self._h = None
 
     def __del__(self):
-        self.close()
+        if capi is not None:      # (None while the interpreter ends)
+            self.close()
