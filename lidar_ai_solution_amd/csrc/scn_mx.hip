@@ -382,15 +382,17 @@ __global__ __launch_bounds__(512) void k_mx_product_few(const ProductArgs p) {
   }
 }
 
-// Bias, ReLU, residual and store of 8 consecutive channels of one row (one 16-byte store in fp16, two in fp32; rows of any
-// alignment).
-__device__ __forceinline__ void product_store8(const ProductArgs& p, uint32_t i, uint32_t j, float (&y)[8]) {
+// Bias, ReLU, residual and store of 8 consecutive channels of one row, from LDS (one 16-byte store in fp16, two in fp32;
+// rows of any alignment).
+__device__ __forceinline__ void product_store8(const ProductArgs& p, uint32_t i, uint32_t j, const float* src) {
   if (j + 8 > p.n) {
-#pragma unroll
-    for (int q = 0; q < 8; ++q)
-      if (j + q < p.n) product_store(p, i, j + q, y[q]);
+#pragma unroll 1
+    for (uint32_t q = 0; j + q < p.n; ++q) product_store(p, i, j + q, src[q]);
     return;
   }
+  float y[8];
+  *reinterpret_cast<v4f*>(y) = *reinterpret_cast<const v4f*>(src);
+  *reinterpret_cast<v4f*>(y + 4) = *reinterpret_cast<const v4f*>(src + 4);
   if (p.bias) {
     if (p.bias_fp32) {
       float b[8];
@@ -449,46 +451,16 @@ __device__ __forceinline__ void product_store8(const ProductArgs& p, uint32_t i,
 // Rows beyond the last are read as the last one and not stored; blocks beyond the last come from a page of zeros.
 __device__ uint4 g_mx_zero[1];   // (device globals are zeroed)
 
-typedef const __attribute__((address_space(1))) void* mx_gptr;
 typedef __attribute__((address_space(3))) void* mx_lptr;
 
-template <int TN, int TM>
-__device__ __forceinline__ void mx_read_operands(uint32_t addr, v4i (&w)[TN], v4i (&x)[TM], uint32_t x_addr) {
-  // one block with its own wait: the outputs are complete when it ends
-  if constexpr (TN == 4 && TM == 2)
-    asm volatile("ds_read_b128 %0, %6\n\tds_read_b128 %4, %7\n\tds_read_b128 %1, %6 offset:4096\n\tds_read_b128 %5, %7 offset:4096\n\t"
-                 "ds_read_b128 %2, %6 offset:8192\n\tds_read_b128 %3, %6 offset:12288\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(x[0]), "=&v"(x[1])
-                 : "v"(addr), "v"(x_addr)
-                 : "memory");
-  else if constexpr (TN == 2 && TM == 2)
-    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %2, %5\n\tds_read_b128 %1, %4 offset:4096\n\tds_read_b128 %3, %5 offset:4096\n\t"
-                 "s_waitcnt lgkmcnt(0)"
-                 : "=&v"(w[0]), "=&v"(w[1]), "=&v"(x[0]), "=&v"(x[1])
-                 : "v"(addr), "v"(x_addr)
-                 : "memory");
-  else
-    asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(w[0]), "=&v"(x[0])
-                 : "v"(addr), "v"(x_addr)
-                 : "memory");
+// 64 x 16 (or 64 x 4) bytes from memory to LDS, lane l's to base + 16 l (4 l).  Written in assembly so that the compiler's
+// own LDS reads are not ordered after every load in flight (it would drain them all); the waits are the explicit counts
+// in the kernel.  The instruction takes its LDS address from m0, which needs one wait state after it is written.
+__device__ __forceinline__ void mx_load16_lds(const void* src, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(base) : "memory", "m0");
 }
-
-template <int N>
-__device__ __forceinline__ void mx_read_scales(uint32_t addr, uint2 (&s)[N]) {
-  uint64_t t[N];
-  if constexpr (N == 4)
-    asm volatile("ds_read_b64 %0, %4\n\tds_read_b64 %1, %4 offset:256\n\tds_read_b64 %2, %4 offset:512\n\tds_read_b64 %3, %4 offset:768\n\t"
-                 "s_waitcnt lgkmcnt(0)"
-                 : "=&v"(t[0]), "=&v"(t[1]), "=&v"(t[2]), "=&v"(t[3])
-                 : "v"(addr)
-                 : "memory");
-  else if constexpr (N == 2)
-    asm volatile("ds_read_b64 %0, %2\n\tds_read_b64 %1, %2 offset:256\n\ts_waitcnt lgkmcnt(0)" : "=&v"(t[0]), "=&v"(t[1]) : "v"(addr) : "memory");
-  else
-    asm volatile("ds_read_b64 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(t[0]) : "v"(addr) : "memory");
-#pragma unroll
-  for (int i = 0; i < N; ++i) s[i] = make_uint2((uint32_t)t[i], (uint32_t)(t[i] >> 32));
+__device__ __forceinline__ void mx_load4_lds(const void* src, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(base) : "memory", "m0");
 }
 
 // (the byte of the scale registers is an immediate of the instruction)
@@ -557,17 +529,16 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
     }
   }
   const uint32_t stages = (p.kb + 7) / 8;
+  const uint32_t base = (uint32_t)(uintptr_t)(mx_lptr)lds;
   auto load = [&](uint32_t st) {
-    char* buf = lds + (st & 1) * STAGE;
+    const uint32_t buf = __builtin_amdgcn_readfirstlane(base + (st & 1) * STAGE);
     const bool in = st * 8 + cblk < p.kb;
 #pragma unroll
-    for (int q = 0; q < CODE_LOADS; ++q)
-      __builtin_amdgcn_global_load_lds((mx_gptr)(in ? csrc[q] + (size_t)st * 128 : zero), (mx_lptr)(buf + (q * WAVES + wave) * 1024), 16, 0, 0);
+    for (int q = 0; q < CODE_LOADS; ++q) mx_load16_lds(in ? csrc[q] + (size_t)st * 128 : zero, buf + (q * WAVES + wave) * 1024);
     const bool sin = st * 8 + (lane & 1) * 4 < p.kb;
 #pragma unroll
     for (int q = 0; q < SCALE_LOADS; ++q)
-      __builtin_amdgcn_global_load_lds((mx_gptr)(sin ? ssrc[q] + (size_t)st * 8 : zero),
-                                       (mx_lptr)(buf + (BN + BM) * 128 + (q * WAVES + wave) * 256), 4, 0, 0);
+      mx_load4_lds(sin ? ssrc[q] + (size_t)st * 8 : zero, buf + (BN + BM) * 128 + (q * WAVES + wave) * 256);
   };
 
   v16f acc[TN][TM];
@@ -579,11 +550,38 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
       for (int j = 0; j < 16; ++j) acc[a][b][j] = 0.f;
 
   const int wn = wave % T::WN, wm = wave / T::WN;
-  const uint32_t base = (uint32_t)(uintptr_t)(mx_lptr)lds;
   const uint32_t w_row = wn * 32 * TN + ln, x_row = BN + wm * 32 * TM + ln;
   const uint32_t swz = (ln >> 1) & 7;
+  v4i w[2][TN], x[2][TM];
+  uint2 ws[TN], xs[TM];
+  const char* sb = nullptr;
+  // operands of step S (64 channels) of the stage at sb
+  auto read = [&](int S, v4i(&wv)[TN], v4i(&xv)[TM]) {
+    const uint32_t pos = ((2 * S + lh) ^ swz) * 16;
+#pragma unroll
+    for (int a = 0; a < TN; ++a) wv[a] = *reinterpret_cast<const v4i*>(sb + (w_row + 32 * a) * 128 + pos);
+#pragma unroll
+    for (int b = 0; b < TM; ++b) xv[b] = *reinterpret_cast<const v4i*>(sb + (x_row + 32 * b) * 128 + pos);
+  };
+  // scales of a stage; blocks 2 s + lh of step s are bytes 0 and 2 of the two words after a shift by lh bytes
+  auto read_scales = [&](uint32_t mask0, uint32_t mask1) {
+#pragma unroll
+    for (int a = 0; a < TN; ++a) {
+      const uint2 v = *reinterpret_cast<const uint2*>(sb + (BN + BM) * 128 + (w_row + 32 * a) * 8);
+      ws[a] = make_uint2((v.x & mask0) >> (8 * lh), (v.y & mask1) >> (8 * lh));
+    }
+#pragma unroll
+    for (int b = 0; b < TM; ++b) {
+      const uint2 v = *reinterpret_cast<const uint2*>(sb + (BN + BM) * 128 + (x_row + 32 * b) * 8);
+      xs[b] = make_uint2((v.x & mask0) >> (8 * lh), (v.y & mask1) >> (8 * lh));
+    }
+  };
+#define SCN_MX_MULTIPLY(BUF, SEL, WORD)                                                            \
+  _Pragma("unroll") for (int a = 0; a < TN; ++a) _Pragma("unroll") for (int b = 0; b < TM; ++b)    \
+      acc[a][b] = mx_mma32_sel<SEL>(w[BUF][a], ws[a].WORD, x[BUF][b], xs[b].WORD, acc[a][b]);
+  const uint32_t full = p.kb / 8;   // stages of 8 blocks; the last one may be shorter
   load(0);
-  for (uint32_t st = 0; st < stages; ++st) {
+  for (uint32_t st = 0; st < full; ++st) {
     if (st + 1 < stages) {
       load(st + 1);
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CODE_LOADS + SCALE_LOADS) : "memory");
@@ -591,33 +589,51 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
     __builtin_amdgcn_s_barrier();
-    const uint32_t sb = base + (st & 1) * STAGE;
-    const uint32_t left = p.kb - st * 8;   // blocks from here on
-    const uint32_t mask0 = left >= 4 ? ~0u : (1u << (8 * left)) - 1u;
-    const uint32_t mask1 = left >= 8 ? ~0u : left > 4 ? (1u << (8 * (left - 4))) - 1u : 0u;
-    uint2 ws[TN], xs[TM];
-    mx_read_scales<TN>(sb + (BN + BM) * 128 + w_row * 8, ws);
-    mx_read_scales<TM>(sb + (BN + BM) * 128 + x_row * 8, xs);
-    // blocks 2 s + lh of step s: bytes 0 and 2 of the two words after a shift by lh bytes
-#pragma unroll
-    for (int a = 0; a < TN; ++a) ws[a] = make_uint2((ws[a].x & mask0) >> (8 * lh), (ws[a].y & mask1) >> (8 * lh));
-#pragma unroll
-    for (int b = 0; b < TM; ++b) xs[b] = make_uint2((xs[b].x & mask0) >> (8 * lh), (xs[b].y & mask1) >> (8 * lh));
-#define SCN_MX_STEP(S, SEL, WORD)                                                                  \
-  if (2 * (S) < left) {                                                                            \
-    v4i w[TN], x[TM];                                                                              \
-    const uint32_t pos = ((2 * (S) + lh) ^ swz) * 16;                                              \
-    mx_read_operands<TN, TM>(sb + w_row * 128 + pos, w, x, sb + x_row * 128 + pos);                \
-    _Pragma("unroll") for (int a = 0; a < TN; ++a) _Pragma("unroll") for (int b = 0; b < TM; ++b)  \
-        acc[a][b] = mx_mma32_sel<SEL>(w[a], ws[a].WORD, x[b], xs[b].WORD, acc[a][b]);              \
-  }
-    SCN_MX_STEP(0, 0, x)
-    SCN_MX_STEP(1, 2, x)
-    SCN_MX_STEP(2, 0, y)
-    SCN_MX_STEP(3, 2, y)
-#undef SCN_MX_STEP
+    asm volatile("" ::: "memory");
+    sb = lds + (st & 1) * STAGE;
+    // the operands of a step are read behind the matrix instructions of the step before it
+    read_scales(~0u, ~0u);
+    read(0, w[0], x[0]);
+    read(1, w[1], x[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    SCN_MX_MULTIPLY(0, 0, x)
+    __builtin_amdgcn_sched_barrier(0);
+    read(2, w[0], x[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    SCN_MX_MULTIPLY(1, 2, x)
+    __builtin_amdgcn_sched_barrier(0);
+    read(3, w[1], x[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    SCN_MX_MULTIPLY(0, 0, y)
+    SCN_MX_MULTIPLY(1, 2, y)
+    asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
   }
+  if (full < stages) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    sb = lds + (full & 1) * STAGE;
+    const uint32_t left = p.kb - full * 8;   // 1 .. 7 blocks
+    read_scales(left >= 4 ? ~0u : (1u << (8 * left)) - 1u, left > 4 ? (1u << (8 * (left - 4))) - 1u : 0u);
+    read(0, w[0], x[0]);
+    SCN_MX_MULTIPLY(0, 0, x)
+    if (left > 2) {
+      read(1, w[0], x[0]);
+      SCN_MX_MULTIPLY(0, 2, x)
+    }
+    if (left > 4) {
+      read(2, w[0], x[0]);
+      SCN_MX_MULTIPLY(0, 0, y)
+    }
+    if (left > 6) {
+      read(3, w[0], x[0]);
+      SCN_MX_MULTIPLY(0, 2, y)
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+  }
+#undef SCN_MX_MULTIPLY
   // Store through LDS (wave-private, 32 rows at a time): a lane of the accumulators holds 4 consecutive channels of one
   // row, a store wants whole 128-byte lines of a row.
   float* buf = reinterpret_cast<float*>(lds) + wave * 32 * T::PAD;
@@ -632,12 +648,8 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
             v4f{acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]};
     const uint32_t row0 = i0 + wm * 32 * TM + b * 32, ch = n0 + wn * 32 * TN + (lane % LPR) * 8;
 #pragma unroll 2
-    for (int r = lane / LPR; r < 32; r += RPP) {
-      float y[8];
-      *reinterpret_cast<v4f*>(y) = *reinterpret_cast<const v4f*>(buf + r * T::PAD + (lane % LPR) * 8);
-      *reinterpret_cast<v4f*>(y + 4) = *reinterpret_cast<const v4f*>(buf + r * T::PAD + (lane % LPR) * 8 + 4);
-      if (row0 + r < m && ch < p.n) product_store8(p, row0 + r, ch, y);
-    }
+    for (int r = lane / LPR; r < 32; r += RPP)
+      if (row0 + r < m && ch < p.n) product_store8(p, row0 + r, ch, buf + r * T::PAD + (lane % LPR) * 8);
   }
 }
 
