@@ -448,19 +448,17 @@ __device__ __forceinline__ void product_store8(const ProductArgs& p, uint32_t i,
 //   so the order is obtained by permuting which block a lane fetches.
 //   A wave owns TN x TM tiles of 32 x 32: per matrix instruction of 64 channels it reads (TN + TM) KB from LDS for TN * TM
 //   products.
-// Rows beyond the last are read as the last one and not stored; blocks beyond the last come from a page of zeros.
-__device__ uint4 g_mx_zero[1];   // (device globals are zeroed)
-
+// Rows beyond the last are read as the last one and not stored.
 typedef __attribute__((address_space(3))) void* mx_lptr;
 
 // 64 x 16 (or 64 x 4) bytes from memory to LDS, lane l's to base + 16 l (4 l).  Written in assembly so that the compiler's
 // own LDS reads are not ordered after every load in flight (it would drain them all); the waits are the explicit counts
-// in the kernel.  The instruction takes its LDS address from m0, which needs one wait state after it is written.
-__device__ __forceinline__ void mx_load16_lds(const void* src, uint32_t base) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(base) : "memory", "m0");
+// in the kernel.  The address is a wave's base with a 32-bit offset per lane.  The instruction takes its LDS address from m0, which needs one wait state after it is written.
+__device__ __forceinline__ void mx_load16_lds(const uint8_t* src, uint32_t offset, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(src), "s"(base) : "memory", "m0");
 }
-__device__ __forceinline__ void mx_load4_lds(const void* src, uint32_t base) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(base) : "memory", "m0");
+__device__ __forceinline__ void mx_load4_lds(const uint8_t* src, uint32_t offset, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(src), "s"(base) : "memory", "m0");
 }
 
 // (the byte of the scale registers is an immediate of the instruction)
@@ -504,41 +502,42 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
   const uint32_t i0 = tm * BM, n0 = tn * BN;
   if (i0 >= m) return;
 
-  // what this lane fetches: code load q covers 8 rows (lane / 8), position lane % 8; scale load q 32 rows (lane / 2)
-  const uint8_t* csrc[CODE_LOADS];
-  const uint8_t* ssrc[SCALE_LOADS];
-  const uint8_t* zero = reinterpret_cast<const uint8_t*>(g_mx_zero);
-  uint32_t cblk;   // block of a stage this lane fetches (the same for every load: rows advance by multiples of 16)
-  {
-    static_assert(WAVES % 2 == 0, "rows of one lane differ by multiples of 16");
-    const int r0 = wave * 8 + (lane >> 3);
-    cblk = (lane & 7) ^ ((r0 >> 1) & 7);
+  // What this lane fetches: code load q covers 8 rows (lane / 8), position lane % 8; scale load q 32 rows (lane / 2).  A wave's
+  // load is all weights or all rows, so an address is a wave's base, which advances from stage to stage, and a lane's offset.
+  static_assert(BN % (WAVES * 8) == 0 && WAVES % 2 == 0, "code loads are weights or rows; rows of one lane differ by multiples of 16");
+  uint32_t coff[CODE_LOADS], soff[SCALE_LOADS];
+  const uint8_t* wcode = p.b + (size_t)n0 * p.b_ld;
+  const uint8_t* xcode = (const uint8_t*)p.a + (size_t)i0 * p.a_ld;
+  const uint8_t* wscale = p.bs + (size_t)n0 * p.bs_ld;
+  const uint8_t* xscale = p.as + (size_t)i0 * p.as_ld;
+  const uint32_t last_w = p.n - 1 - n0, last_x = m - 1 - i0;   // rows of this tile that exist
+  const uint32_t cblk = (lane & 7) ^ (((wave * 8 + (lane >> 3)) >> 1) & 7);   // block of a stage this lane fetches
 #pragma unroll
-    for (int q = 0; q < CODE_LOADS; ++q) {
-      const uint32_t r = q * WAVES * 8 + r0;   // BN is a multiple of WAVES * 8: a load is all weights or all rows
-      const bool is_w = q * WAVES * 8 < BN;
-      const size_t row = is_w ? min(n0 + r, p.n - 1) : min(i0 + r - BN, m - 1);
-      csrc[q] = (is_w ? p.b + row * p.b_ld : (const uint8_t*)p.a + row * p.a_ld) + cblk * 16;
-    }
-#pragma unroll
-    for (int q = 0; q < SCALE_LOADS; ++q) {
-      const uint32_t r = q * WAVES * 32 + wave * 32 + (lane >> 1);
-      const bool is_w = r < BN;
-      const size_t row = is_w ? min(n0 + r, p.n - 1) : min(i0 + r - BN, m - 1);
-      ssrc[q] = (is_w ? p.bs + row * p.bs_ld : p.as + row * p.as_ld) + (lane & 1) * 4;
-    }
+  for (int q = 0; q < CODE_LOADS; ++q) {
+    const uint32_t r = q * WAVES * 8 + wave * 8 + (lane >> 3);
+    coff[q] = (q * WAVES * 8 < BN ? min(r, last_w) * p.b_ld : min(r - BN, last_x) * p.a_ld) + cblk * 16;
   }
-  const uint32_t stages = (p.kb + 7) / 8;
-  const uint32_t base = (uint32_t)(uintptr_t)(mx_lptr)lds;
-  auto load = [&](uint32_t st) {
-    const uint32_t buf = __builtin_amdgcn_readfirstlane(base + (st & 1) * STAGE);
-    const bool in = st * 8 + cblk < p.kb;
+  auto scale_is_w = [&](int q) { return q * WAVES * 32 + wave * 32 < BN; };   // (uniform)
 #pragma unroll
-    for (int q = 0; q < CODE_LOADS; ++q) mx_load16_lds(in ? csrc[q] + (size_t)st * 128 : zero, buf + (q * WAVES + wave) * 1024);
-    const bool sin = st * 8 + (lane & 1) * 4 < p.kb;
+  for (int q = 0; q < SCALE_LOADS; ++q) {
+    const uint32_t r = q * WAVES * 32 + wave * 32 + (lane >> 1);
+    soff[q] = (scale_is_w(q) ? min(r, last_w) * p.bs_ld : min(r - BN, last_x) * p.as_ld) + (lane & 1) * 4;
+  }
+  const uint32_t stages = (p.kb + 7) / 8;   // of 8 blocks; the last one may be shorter
+  const uint32_t base = (uint32_t)(uintptr_t)(mx_lptr)lds;
+  // Loads [from, to) of a wave's CODE_LOADS + SCALE_LOADS of stage st.  In a stage of fewer than 8 blocks a lane whose block
+  // does not exist fetches the first one instead: the masked scales (2^-127 on both sides) take it out of the sums.
+  auto load = [&](uint32_t st, int from, int to) {
+    const uint32_t buf = __builtin_amdgcn_readfirstlane(base + (st & 1) * STAGE);
+    const uint32_t cback = st * 8 + cblk < p.kb ? 0u : cblk * 16, sback = st * 8 + (lane & 1) * 4 < p.kb ? 0u : 4u;
+#pragma unroll
+    for (int q = 0; q < CODE_LOADS; ++q)
+      if (q >= from && q < to)
+        mx_load16_lds((q * WAVES * 8 < BN ? wcode : xcode) + (size_t)st * 128, coff[q] - cback, buf + (q * WAVES + wave) * 1024);
 #pragma unroll
     for (int q = 0; q < SCALE_LOADS; ++q)
-      mx_load4_lds(sin ? ssrc[q] + (size_t)st * 8 : zero, buf + (BN + BM) * 128 + (q * WAVES + wave) * 256);
+      if (CODE_LOADS + q >= from && CODE_LOADS + q < to)
+        mx_load4_lds((scale_is_w(q) ? wscale : xscale) + (size_t)st * 8, soff[q] - sback, buf + (BN + BM) * 128 + (q * WAVES + wave) * 256);
   };
 
   v16f acc[TN][TM];
@@ -579,43 +578,41 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
 #define SCN_MX_MULTIPLY(BUF, SEL, WORD)                                                            \
   _Pragma("unroll") for (int a = 0; a < TN; ++a) _Pragma("unroll") for (int b = 0; b < TM; ++b)    \
       acc[a][b] = mx_mma32_sel<SEL>(w[BUF][a], ws[a].WORD, x[BUF][b], xs[b].WORD, acc[a][b]);
-  const uint32_t full = p.kb / 8;   // stages of 8 blocks; the last one may be shorter
-  load(0);
-  for (uint32_t st = 0; st < full; ++st) {
-    if (st + 1 < stages) {
-      load(st + 1);
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CODE_LOADS + SCALE_LOADS) : "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
+  // A stage: wait for its loads, one barrier (after it every wave has also finished with the other buffer), then the
+  // products, with the next stage's loads issued between them (all at once they would fill the memory pipe's queue and
+  // hold up the matrix instructions behind it) and each step's operands read behind the products of the step before.
+  constexpr int LOADS = CODE_LOADS + SCALE_LOADS;
+  load(0, 0, LOADS);
+  for (uint32_t st = 0; st + 1 < stages; ++st) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     sb = lds + (st & 1) * STAGE;
-    // the operands of a step are read behind the matrix instructions of the step before it
     read_scales(~0u, ~0u);
     read(0, w[0], x[0]);
     read(1, w[1], x[1]);
     __builtin_amdgcn_sched_barrier(0);
+    load(st + 1, 0, LOADS / 3);
     SCN_MX_MULTIPLY(0, 0, x)
     __builtin_amdgcn_sched_barrier(0);
     read(2, w[0], x[0]);
     __builtin_amdgcn_sched_barrier(0);
+    load(st + 1, LOADS / 3, LOADS * 2 / 3);
     SCN_MX_MULTIPLY(1, 2, x)
     __builtin_amdgcn_sched_barrier(0);
     read(3, w[1], x[1]);
     __builtin_amdgcn_sched_barrier(0);
+    load(st + 1, LOADS * 2 / 3, LOADS);
     SCN_MX_MULTIPLY(0, 0, y)
     SCN_MX_MULTIPLY(1, 2, y)
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
   }
-  if (full < stages) {
+  {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    sb = lds + (full & 1) * STAGE;
-    const uint32_t left = p.kb - full * 8;   // 1 .. 7 blocks
-    read_scales(left >= 4 ? ~0u : (1u << (8 * left)) - 1u, left > 4 ? (1u << (8 * (left - 4))) - 1u : 0u);
+    sb = lds + ((stages - 1) & 1) * STAGE;
+    const uint32_t left = p.kb - (stages - 1) * 8;   // 1 .. 8 blocks
+    read_scales(left >= 4 ? ~0u : (1u << (8 * left)) - 1u, left >= 8 ? ~0u : left > 4 ? (1u << (8 * (left - 4))) - 1u : 0u);
     read(0, w[0], x[0]);
     SCN_MX_MULTIPLY(0, 0, x)
     if (left > 2) {
@@ -630,10 +627,10 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
       read(3, w[0], x[0]);
       SCN_MX_MULTIPLY(0, 2, y)
     }
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
   }
 #undef SCN_MX_MULTIPLY
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
   // Store through LDS (wave-private, 32 rows at a time): a lane of the accumulators holds 4 consecutive channels of one
   // row, a store wants whole 128-byte lines of a row.
   float* buf = reinterpret_cast<float*>(lds) + wave * 32 * T::PAD;
@@ -657,6 +654,8 @@ template <int BN, int BM, int TN, int TM>
 static int launch_product(const ProductArgs& p, hipStream_t stream) {
   using T = ProductTile<BN, BM, TN, TM>;
   const uint64_t tn = ((uint64_t)p.n + BN - 1) / BN, tm = ((uint64_t)p.m + BM - 1) / BM;
+  SCN_REQUIRE((uint64_t)std::max(std::max(p.a_ld, p.b_ld), std::max(p.as_ld, p.bs_ld)) * 256 < (1ull << 32), SCN_ERR_UNSUPPORTED,
+              "mx_product: rows more than 16 MB apart");
   SCN_REQUIRE(tn * tm < (1ull << 27), SCN_ERR_UNSUPPORTED, "mx_product: %u x %u outputs are too many for one call", p.m, p.n);
   const size_t lds = T::lds((p.kb + 7) / 8);
   hipLaunchKernelGGL((k_mx_product_lds<BN, BM, TN, TM>), dim3((unsigned)((tn * tm + 7) / 8 * 8)), dim3(64 * T::WAVES), lds, stream, p,
