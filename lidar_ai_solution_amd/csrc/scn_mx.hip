@@ -439,15 +439,18 @@ __device__ __forceinline__ void product_store8(const ProductArgs& p, uint32_t i,
   }
 }
 
-// Any number of rows.  A workgroup of 4 * WN * WM... waves owns BN output channels x BM rows; both operands are staged
-// through LDS, 256 channels (8 blocks = 128 code bytes and 8 scale bytes per row) at a time, by loads that go straight to
-// LDS, two stages deep.
-//   LDS of a stage: codes of the BN weight rows, codes of the BM rows (128 bytes each), then their scales (8 bytes each).
-//   Block c of row r lies at position c ^ (r / 2) % 8 of its row, so that the 16-byte operand reads of 16 neighbouring rows
-//   touch all 64 banks once (rows of 128 bytes: two rows fill the banks).  The hardware places lane l's bytes at base + 16 l,
-//   so the order is obtained by permuting which block a lane fetches.
-//   A wave owns TN x TM tiles of 32 x 32: per matrix instruction of 64 channels it reads (TN + TM) KB from LDS for TN * TM
-//   products.
+// Any number of rows.  A workgroup owns BN output channels x BM rows, a wave of it TN x TM tiles of 32 x 32; both operands are
+// staged through LDS, 256 channels (8 blocks = 128 code bytes) at a time, by loads that go straight to LDS, two stages deep.
+//   LDS of a stage: codes of the BN weight rows, then of the BM rows (128 bytes each).  Block c of row r lies at position
+//   c ^ (r / 2) % 8 of its row, so that the 16-byte operand reads of 16 neighbouring rows touch all 64 banks once.  The hardware
+//   places lane l's bytes at base + 16 l, so the order is obtained by permuting which block a lane fetches.
+//   Scales are fetched for 2 stages at once (16 bytes per row), two such spans.
+// What bounds it is the memory pipe next to the matrix cores: it counts requests, a line of 128 bytes as much as 4 bytes of one,
+// so codes come in whole lines and scales in spans.  (8192 cubed with 64-byte code rows and scales word by word: 350 us;
+// 64-byte rows and spans: 291 us.)
+// The last operands of a stage are multiplied behind the barrier in front of the next one, while that one's first operands are
+// read, so the matrix pipe does not wait for LDS there.
+//   Per matrix instruction of 64 channels a wave reads (TN + TM) KB / (TN * TM) from LDS.
 // Rows beyond the last are read as the last one and not stored.
 typedef __attribute__((address_space(3))) void* mx_lptr;
 
@@ -471,10 +474,10 @@ __device__ __forceinline__ v16f mx_mma32_sel(const v4i& a, uint32_t sa, const v4
 template <int BN, int BM, int TN, int TM>
 struct ProductTile {
   static constexpr int WN = BN / (32 * TN), WM = BM / (32 * TM), WAVES = WN * WM;
-  static constexpr int STAGE = (BN + BM) * 136;                       // bytes of LDS per stage
+  static constexpr int STAGE = (BN + BM) * 128, SPAN = (BN + BM) * 16;   // bytes of LDS per stage of codes, per span of scales
   static constexpr int PAD = 32 * TN + 4;                             // floats per row of the store buffer
   static constexpr int STORE = WAVES * 32 * PAD * 4;
-  static size_t lds(uint32_t stages) { return std::max<size_t>((stages > 1 ? 2 : 1) * (size_t)STAGE, STORE); }
+  static size_t lds(uint32_t stages) { return std::max<size_t>((stages > 1 ? 2 : 1) * (size_t)STAGE + (stages > 2 ? 2 : 1) * SPAN, STORE); }
 };
 
 template <int BN, int BM, int TN, int TM>
@@ -484,9 +487,10 @@ template <int BN, int BM, int TN, int TM>
 __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_product_lds(const ProductArgs p, uint32_t tiles_n,
                                                                                               uint32_t tiles_m) {
   using T = ProductTile<BN, BM, TN, TM>;
-  constexpr int WAVES = T::WAVES, STAGE = T::STAGE;
-  constexpr int CODE_LOADS = (BN + BM) / 8 / WAVES, SCALE_LOADS = (BN + BM) / 32 / WAVES;   // wave loads per stage
-  static_assert(CODE_LOADS * 8 * WAVES == BN + BM && SCALE_LOADS * 32 * WAVES == BN + BM, "loads do not divide");
+  constexpr int WAVES = T::WAVES, STAGE = T::STAGE, SPAN = T::SPAN;
+  constexpr int LOADS = (BN + BM) / 8 / WAVES;   // wave loads per stage of codes
+  static_assert(LOADS * 8 * WAVES == BN + BM && BN % (WAVES * 8) == 0 && WAVES % 2 == 0 && BN % 64 == 0 && BN + BM <= WAVES * 64,
+                "a wave's load is all weights or all rows, and one load per wave fetches a span of scales");
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, lh = lane >> 5;
@@ -502,42 +506,48 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
   const uint32_t i0 = tm * BM, n0 = tn * BN;
   if (i0 >= m) return;
 
-  // What this lane fetches: code load q covers 8 rows (lane / 8), position lane % 8; scale load q 32 rows (lane / 2).  A wave's
-  // load is all weights or all rows, so an address is a wave's base, which advances from stage to stage, and a lane's offset.
-  static_assert(BN % (WAVES * 8) == 0 && WAVES % 2 == 0, "code loads are weights or rows; rows of one lane differ by multiples of 16");
-  uint32_t coff[CODE_LOADS], soff[SCALE_LOADS];
+  // What this lane fetches: code load q covers 8 rows (lane / 8), position lane % 8; the scale load 64 rows.  A wave's load is
+  // all weights or all rows, so an address is a wave's base, which advances from stage to stage, and a lane's offset.
+  uint32_t coff[LOADS];
   const uint8_t* wcode = p.b + (size_t)n0 * p.b_ld;
   const uint8_t* xcode = (const uint8_t*)p.a + (size_t)i0 * p.a_ld;
-  const uint8_t* wscale = p.bs + (size_t)n0 * p.bs_ld;
-  const uint8_t* xscale = p.as + (size_t)i0 * p.as_ld;
   const uint32_t last_w = p.n - 1 - n0, last_x = m - 1 - i0;   // rows of this tile that exist
-  const uint32_t cblk = (lane & 7) ^ (((wave * 8 + (lane >> 3)) >> 1) & 7);   // block of a stage this lane fetches
+  const uint32_t cblk = (lane & 7) ^ ((wave * 4 + (lane >> 4)) & 7);   // block of a stage this lane fetches
 #pragma unroll
-  for (int q = 0; q < CODE_LOADS; ++q) {
+  for (int q = 0; q < LOADS; ++q) {
     const uint32_t r = q * WAVES * 8 + wave * 8 + (lane >> 3);
     coff[q] = (q * WAVES * 8 < BN ? min(r, last_w) * p.b_ld : min(r - BN, last_x) * p.a_ld) + cblk * 16;
   }
-  auto scale_is_w = [&](int q) { return q * WAVES * 32 + wave * 32 < BN; };   // (uniform)
-#pragma unroll
-  for (int q = 0; q < SCALE_LOADS; ++q) {
-    const uint32_t r = q * WAVES * 32 + wave * 32 + (lane >> 1);
-    soff[q] = (scale_is_w(q) ? min(r, last_w) * p.bs_ld : min(r - BN, last_x) * p.as_ld) + (lane & 1) * 4;
-  }
-  const uint32_t stages = (p.kb + 7) / 8;   // of 8 blocks; the last one may be shorter
+  const uint32_t srow = (wave * 64) % (BN + BM);               // (the small tile has fewer rows than lanes: some are loaded twice)
+  const bool s_is_w = srow < BN;
+  const uint8_t* sbase = s_is_w ? p.bs + (size_t)n0 * p.bs_ld : p.as + (size_t)i0 * p.as_ld;
+  const uint32_t s_ld = s_is_w ? p.bs_ld : p.as_ld, srow0 = s_is_w ? srow : srow - BN, last_s = s_is_w ? last_w : last_x;
+  const uint32_t soff = min(srow0 + lane, last_s) * s_ld;
+  const uint32_t stages = (p.kb + 7) / 8, words = (p.kb + 3) / 4;   // stages of 8 blocks, scale words of 4; the last may be shorter
   const uint32_t base = (uint32_t)(uintptr_t)(mx_lptr)lds;
-  // Loads [from, to) of a wave's CODE_LOADS + SCALE_LOADS of stage st.  In a stage of fewer than 8 blocks a lane whose block
-  // does not exist fetches the first one instead: the masked scales (2^-127 on both sides) take it out of the sums.
+  const uint32_t span0 = (stages > 1 ? 2 : 1) * STAGE;              // LDS offset of the scales
+  // Loads [from, to) of a wave's LOADS of stage st.  In a stage of fewer than 8 blocks a lane whose block does not exist
+  // fetches the first one instead: the masked scales (2^-127 on both sides) take it out of the sums.
   auto load = [&](uint32_t st, int from, int to) {
     const uint32_t buf = __builtin_amdgcn_readfirstlane(base + (st & 1) * STAGE);
-    const uint32_t cback = st * 8 + cblk < p.kb ? 0u : cblk * 16, sback = st * 8 + (lane & 1) * 4 < p.kb ? 0u : 4u;
+    const uint32_t back = st * 8 + cblk < p.kb ? 0u : cblk * 16;
 #pragma unroll
-    for (int q = 0; q < CODE_LOADS; ++q)
+    for (int q = 0; q < LOADS; ++q)
       if (q >= from && q < to)
-        mx_load16_lds((q * WAVES * 8 < BN ? wcode : xcode) + (size_t)st * 128, coff[q] - cback, buf + (q * WAVES + wave) * 1024);
+        mx_load16_lds((q * WAVES * 8 < BN ? wcode : xcode) + (size_t)st * 128, coff[q] - back, buf + (q * WAVES + wave) * 1024);
+  };
+  // Scales of stages 2 t and 2 t + 1: 16 bytes per row in one load, or word by word (4 loads, 16 rows x 4 words each) when the
+  // rows end inside the span; words that do not exist are read as the span's first and never used.
+  auto load_scales = [&](uint32_t t) {
+    const uint32_t buf = __builtin_amdgcn_readfirstlane(base + span0 + (t & 1) * SPAN + srow * 16);
+    if (4 * t + 4 <= words) {
+      mx_load16_lds(sbase + (size_t)t * 16, soff, buf);
+    } else if (4 * t < words) {
+      const uint32_t word = 4 * t + (lane & 3) < words ? (lane & 3) * 4 : 0u;
 #pragma unroll
-    for (int q = 0; q < SCALE_LOADS; ++q)
-      if (CODE_LOADS + q >= from && CODE_LOADS + q < to)
-        mx_load4_lds((scale_is_w(q) ? wscale : xscale) + (size_t)st * 8, soff[q] - sback, buf + (BN + BM) * 128 + (q * WAVES + wave) * 256);
+      for (int q = 0; q < 4; ++q)
+        mx_load4_lds(sbase + (size_t)t * 16, min(srow0 + q * 16 + (lane >> 2), last_s) * s_ld + word, buf + q * 256);
+    }
   };
 
   v16f acc[TN][TM];
@@ -552,83 +562,94 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
   const uint32_t w_row = wn * 32 * TN + ln, x_row = BN + wm * 32 * TM + ln;
   const uint32_t swz = (ln >> 1) & 7;
   v4i w[2][TN], x[2][TM];
-  uint2 ws[TN], xs[TM];
-  const char* sb = nullptr;
-  // operands of step S (64 channels) of the stage at sb
-  auto read = [&](int S, v4i(&wv)[TN], v4i(&xv)[TM]) {
+  uint2 ws[TN], xs[TM], ws1[TN], xs1[TM];
+  // operands of step S (64 channels) of stage st
+  auto read = [&](uint32_t st, int S, v4i(&wv)[TN], v4i(&xv)[TM]) {
+    const char* sb = lds + (st & 1) * STAGE;
     const uint32_t pos = ((2 * S + lh) ^ swz) * 16;
 #pragma unroll
     for (int a = 0; a < TN; ++a) wv[a] = *reinterpret_cast<const v4i*>(sb + (w_row + 32 * a) * 128 + pos);
 #pragma unroll
     for (int b = 0; b < TM; ++b) xv[b] = *reinterpret_cast<const v4i*>(sb + (x_row + 32 * b) * 128 + pos);
   };
-  // scales of a stage; blocks 2 s + lh of step s are bytes 0 and 2 of the two words after a shift by lh bytes
-  auto read_scales = [&](uint32_t mask0, uint32_t mask1) {
+  // the scale words of a stage; take_scales: blocks 2 s + lh of step s are bytes 0 and 2 of the words after a shift by lh bytes
+  auto read_scales = [&](uint32_t st) {
+    const char* sb = lds + span0 + ((st >> 1) & 1) * SPAN + (st & 1) * 8;
 #pragma unroll
-    for (int a = 0; a < TN; ++a) {
-      const uint2 v = *reinterpret_cast<const uint2*>(sb + (BN + BM) * 128 + (w_row + 32 * a) * 8);
-      ws[a] = make_uint2((v.x & mask0) >> (8 * lh), (v.y & mask1) >> (8 * lh));
-    }
+    for (int a = 0; a < TN; ++a) ws1[a] = *reinterpret_cast<const uint2*>(sb + (w_row + 32 * a) * 16);
 #pragma unroll
-    for (int b = 0; b < TM; ++b) {
-      const uint2 v = *reinterpret_cast<const uint2*>(sb + (BN + BM) * 128 + (x_row + 32 * b) * 8);
-      xs[b] = make_uint2((v.x & mask0) >> (8 * lh), (v.y & mask1) >> (8 * lh));
-    }
+    for (int b = 0; b < TM; ++b) xs1[b] = *reinterpret_cast<const uint2*>(sb + (x_row + 32 * b) * 16);
+  };
+  auto take_scales = [&](uint32_t mask0, uint32_t mask1) {
+#pragma unroll
+    for (int a = 0; a < TN; ++a) ws[a] = make_uint2((ws1[a].x & mask0) >> (8 * lh), (ws1[a].y & mask1) >> (8 * lh));
+#pragma unroll
+    for (int b = 0; b < TM; ++b) xs[b] = make_uint2((xs1[b].x & mask0) >> (8 * lh), (xs1[b].y & mask1) >> (8 * lh));
   };
 #define SCN_MX_MULTIPLY(BUF, SEL, WORD)                                                            \
   _Pragma("unroll") for (int a = 0; a < TN; ++a) _Pragma("unroll") for (int b = 0; b < TM; ++b)    \
       acc[a][b] = mx_mma32_sel<SEL>(w[BUF][a], ws[a].WORD, x[BUF][b], xs[b].WORD, acc[a][b]);
-  // A stage: wait for its loads, one barrier (after it every wave has also finished with the other buffer), then the
-  // products, with the next stage's loads issued between them (all at once they would fill the memory pipe's queue and
-  // hold up the matrix instructions behind it) and each step's operands read behind the products of the step before.
-  constexpr int LOADS = CODE_LOADS + SCALE_LOADS;
+// every load has landed and every wave is done with the other buffer (its operands are in registers)
+#define SCN_MX_BARRIER()                                                  \
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");             \
+  __builtin_amdgcn_s_barrier();                                           \
+  asm volatile("" ::: "memory");
+  // Steps 0 .. 3 of every stage but the last; the products of a stage's step 3 come behind the next barrier (none before the
+  // first: zeros).
+#pragma unroll
+  for (int a = 0; a < TN; ++a) w[1][a] = v4i{0, 0, 0, 0}, ws[a] = make_uint2(0, 0);
+#pragma unroll
+  for (int b = 0; b < TM; ++b) x[1][b] = v4i{0, 0, 0, 0}, xs[b] = make_uint2(0, 0);
+  load_scales(0);
   load(0, 0, LOADS);
-  for (uint32_t st = 0; st + 1 < stages; ++st) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    sb = lds + (st & 1) * STAGE;
-    read_scales(~0u, ~0u);
-    read(0, w[0], x[0]);
-    read(1, w[1], x[1]);
+  uint32_t st = 0;
+#pragma unroll 1
+  for (; st + 1 < stages; ++st) {
+    SCN_MX_BARRIER()
+    if (!(st & 1)) load_scales(st / 2 + 1);
+    read_scales(st);
+    read(st, 0, w[0], x[0]);
     __builtin_amdgcn_sched_barrier(0);
-    load(st + 1, 0, LOADS / 3);
+    load(st + 1, 0, LOADS / 2);
+    SCN_MX_MULTIPLY(1, 2, y)
+    take_scales(~0u, ~0u);
+    __builtin_amdgcn_sched_barrier(0);
+    read(st, 1, w[1], x[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    load(st + 1, LOADS / 2, LOADS);
     SCN_MX_MULTIPLY(0, 0, x)
     __builtin_amdgcn_sched_barrier(0);
-    read(2, w[0], x[0]);
+    read(st, 2, w[0], x[0]);
     __builtin_amdgcn_sched_barrier(0);
-    load(st + 1, LOADS / 3, LOADS * 2 / 3);
     SCN_MX_MULTIPLY(1, 2, x)
     __builtin_amdgcn_sched_barrier(0);
-    read(3, w[1], x[1]);
+    read(st, 3, w[1], x[1]);
     __builtin_amdgcn_sched_barrier(0);
-    load(st + 1, LOADS * 2 / 3, LOADS);
     SCN_MX_MULTIPLY(0, 0, y)
-    SCN_MX_MULTIPLY(1, 2, y)
   }
-  {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    sb = lds + ((stages - 1) & 1) * STAGE;
-    const uint32_t left = p.kb - (stages - 1) * 8;   // 1 .. 8 blocks
-    read_scales(left >= 4 ? ~0u : (1u << (8 * left)) - 1u, left >= 8 ? ~0u : left > 4 ? (1u << (8 * (left - 4))) - 1u : 0u);
-    read(0, w[0], x[0]);
+  SCN_MX_MULTIPLY(1, 2, y)
+  {   // the last stage, of 1 .. 8 blocks
+    SCN_MX_BARRIER()
+    const uint32_t left = p.kb - st * 8;
+    read_scales(st);
+    take_scales(left >= 4 ? ~0u : (1u << (8 * left)) - 1u, left >= 8 ? ~0u : left > 4 ? (1u << (8 * (left - 4))) - 1u : 0u);
+    read(st, 0, w[0], x[0]);
     SCN_MX_MULTIPLY(0, 0, x)
     if (left > 2) {
-      read(1, w[0], x[0]);
+      read(st, 1, w[0], x[0]);
       SCN_MX_MULTIPLY(0, 2, x)
     }
     if (left > 4) {
-      read(2, w[0], x[0]);
+      read(st, 2, w[0], x[0]);
       SCN_MX_MULTIPLY(0, 0, y)
     }
     if (left > 6) {
-      read(3, w[0], x[0]);
+      read(st, 3, w[0], x[0]);
       SCN_MX_MULTIPLY(0, 2, y)
     }
   }
 #undef SCN_MX_MULTIPLY
+#undef SCN_MX_BARRIER
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   // Store through LDS (wave-private, 32 rows at a time): a lane of the accumulators holds 4 consecutive channels of one
