@@ -305,9 +305,9 @@ __device__ __forceinline__ void product_store(const ProductArgs& p, uint32_t i, 
   else ((_Float16*)p.out)[at] = (_Float16)y;
 }
 
-// Codes and scale of block `b` of a row that is not quantised yet, by one lane.
+// Codes and scale byte of block `b` of a row that is not quantised yet, by one thread.
 template <int DT>
-__device__ __forceinline__ uint4 mx_quantize_lane(const typename MxIn<DT>::T* row, uint32_t b, uint32_t c, int* scale) {
+__device__ __forceinline__ uint4 mx_quantize_block_dev(const typename MxIn<DT>::T* row, uint32_t b, uint32_t c, uint32_t* scale) {
   float v[32];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -320,7 +320,7 @@ __device__ __forceinline__ uint4 mx_quantize_lane(const typename MxIn<DT>::T* ro
 #pragma unroll
   for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
   const uint32_t e = mx_scale_byte(top);
-  *scale = (int)e;
+  *scale = e;
   if (e == 255u) return make_uint4(0, 0, 0, 0);
   const float up = __uint_as_float((254u - e) << 23);
   uint32_t w[4];
@@ -334,57 +334,98 @@ __device__ __forceinline__ uint4 mx_quantize_lane(const typename MxIn<DT>::T* ro
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Few rows (m <= 16): bound by reading the weights.  A workgroup owns 16 output channels and all rows; its 8 waves
-// split the channels k between them (contiguous runs of 128) and add their sums in LDS, in wave order.  Rows that are
-// not quantised are quantised by the lane that supplies them (AT = their dtype; SCN_DTYPE_MXFP4: they are).
-template <int AT>
+// Few rows (m <= 16 MT): bound by reading the weights.  A workgroup owns 16 output channels and all rows; its (up to 8) waves
+// split the channels k between them (contiguous runs of 128) and add their sums in LDS, in wave order.  The weights of U runs
+// are requested before anything waits (U KB per wave in flight), so rows that are not quantised yet (AT = their dtype) are
+// quantised into LDS by the whole workgroup while the weights travel.
+// (8192 x 8192 weights, one fp16 row: 21.4 us with a dependent load per run and every wave quantising for itself, 11.9 us so.)
+constexpr uint32_t kFewBlocks = 1024;   // blocks of quantised rows in LDS
+
+template <int AT, int MT, int U>
 __global__ __launch_bounds__(512) void k_mx_product_few(const ProductArgs p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr bool MX = AT == SCN_DTYPE_MXFP4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int lr = lane & 15, lg = lane >> 4;
+  __shared__ uint4 xcodes[MX ? 1 : kFewBlocks];
+  __shared__ uint8_t xscales[MX ? 1 : kFewBlocks];
+  __shared__ float part[8][MT][64][4];
   const uint32_t m = eff_n(p.m_dev, p.m);
   if (m == 0) return;
   const uint32_t n0 = blockIdx.x * 16;
-  const uint32_t brow = min(n0 + lr, p.n - 1), arow = min((uint32_t)lr, m - 1);
+  const uint32_t brow = min(n0 + lr, p.n - 1);
   const uint8_t* bc = p.b + (size_t)brow * p.b_ld;
   const uint8_t* bsc = p.bs + (size_t)brow * p.bs_ld;
-  const uint32_t steps = (p.kb + 3) / 4, per = (steps + 7) / 8;
-  const uint32_t s0 = wave * per, s1 = min(steps, s0 + per);
-  v4f acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (uint32_t s = s0; s < s1; ++s) {
-    const uint32_t blk = 4 * s + lg;
-    uint4 wq = make_uint4(0, 0, 0, 0), xq = make_uint4(0, 0, 0, 0);
-    int ws = 0, xs = 0;
-    if (blk < p.kb) {
-      wq = *reinterpret_cast<const uint4*>(bc + (size_t)blk * 16);
-      ws = bsc[blk];
-      if constexpr (AT == SCN_DTYPE_MXFP4) {
-        xq = *reinterpret_cast<const uint4*>((const uint8_t*)p.a + (size_t)arow * p.a_ld + (size_t)blk * 16);
-        xs = p.as[(size_t)arow * p.as_ld + blk];
-      } else if ((uint32_t)lr < m) {
-        typedef typename MxIn<AT>::T T;
-        xq = mx_quantize_lane<AT>((const T*)p.a + (size_t)arow * p.a_ld, blk, p.k, &xs);
+  uint32_t arow[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) arow[t] = min((uint32_t)(16 * t + lr), m - 1);
+  v4f acc[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
+  const uint32_t runs = (p.kb + 3) / 4, per = (runs + waves - 1) / waves;   // runs of 4 blocks
+  const uint32_t s1 = min(runs, (wave + 1) * per);
+  bool quantised = MX;
+  for (uint32_t s = wave * per; !quantised || s < s1; s += U) {
+    uint4 wq[U], xq[U][MT];
+    uint32_t ws[U], xs[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {   // (a run or block that does not exist reads the row's first block and is masked below)
+      const uint32_t blk = s + u < s1 && 4 * (s + u) + lg < p.kb ? 4 * (s + u) + lg : 0u;
+      wq[u] = *reinterpret_cast<const uint4*>(bc + (size_t)blk * 16);
+      ws[u] = bsc[blk];
+      if constexpr (MX) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          xq[u][t] = *reinterpret_cast<const uint4*>((const uint8_t*)p.a + (size_t)arow[t] * p.a_ld + (size_t)blk * 16);
+          xs[u][t] = p.as[(size_t)arow[t] * p.as_ld + blk];
+        }
       }
     }
-    acc = mx_mma16(wq, ws, xq, xs, acc);
+    if constexpr (!MX) {
+      if (!quantised) {
+        typedef typename MxIn<AT>::T T;
+        for (uint32_t e = threadIdx.x; e < m * p.kb; e += blockDim.x) {
+          const uint32_t row = e / p.kb, b = e - row * p.kb;
+          uint32_t sc;
+          xcodes[e] = mx_quantize_block_dev<AT>((const T*)p.a + (size_t)row * p.a_ld, b, p.k, &sc);
+          xscales[e] = (uint8_t)sc;
+        }
+        __syncthreads();
+        quantised = true;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = s + u < s1 && 4 * (s + u) + lg < p.kb;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        if constexpr (!MX) {
+          const uint32_t e = arow[t] * p.kb + (in ? 4 * (s + u) + lg : 0u);
+          xq[u][t] = xcodes[e];
+          xs[u][t] = xscales[e];
+        }
+        acc[t] = mx_mma16(wq[u], in ? ws[u] : 0u, xq[u][t], in ? xs[u][t] : 0u, acc[t]);
+      }
+    }
   }
-  __shared__ float part[8][64][4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) part[wave][lane][j] = acc[j];
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) part[wave][t][lane][j] = acc[t][j];
   __syncthreads();
-  if (threadIdx.x < 256) {
-    // thread = (row, channel), channels fastest: channel 4 g + j of row r is element j of lane 16 g + r
-    const uint32_t i = threadIdx.x / 16, ch = threadIdx.x % 16;
+  // element = (row, channel), channels fastest: channel 4 g + j of row 16 t + r is element j of lane 16 g + r of tile t
+  for (uint32_t q = threadIdx.x; q < 256u * MT; q += blockDim.x) {
+    const uint32_t i = q / 16, ch = q % 16;
+    if (i >= m || n0 + ch >= p.n) continue;
     float y = 0.f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) y += part[w][(ch / 4) * 16 + i][ch % 4];
-    if (i < m && n0 + ch < p.n) product_store(p, i, n0 + ch, y);
+    for (int w = 0; w < waves; ++w) y += part[w][i / 16][(ch / 4) * 16 + i % 16][ch % 4];
+    product_store(p, i, n0 + ch, y);
   }
 }
 
 // Bias, ReLU, residual and store of 8 consecutive channels of one row, from LDS (one 16-byte store in fp16, two in fp32;
-// rows of any alignment).
-__device__ __forceinline__ void product_store8(const ProductArgs& p, uint32_t i, uint32_t j, const float* src) {
+// rows of any alignment).  PRE: an fp16 residual has been loaded into `pre` already.
+template <bool PRE>
+__device__ __forceinline__ void product_store8(const ProductArgs& p, uint32_t i, uint32_t j, const float* src, const v4u pre) {
   if (j + 8 > p.n) {
 #pragma unroll 1
     for (uint32_t q = 0; j + q < p.n; ++q) product_store(p, i, j + q, src[q]);
@@ -419,7 +460,8 @@ __device__ __forceinline__ void product_store8(const ProductArgs& p, uint32_t i,
       for (int q = 0; q < 8; ++q) y[q] += r[q];
     } else {
       _Float16 r[8];
-      __builtin_memcpy(r, (const _Float16*)p.res + at, 16);
+      if constexpr (PRE) __builtin_memcpy(r, &pre, 16);
+      else __builtin_memcpy(r, (const _Float16*)p.res + at, 16);
 #pragma unroll
       for (int q = 0; q < 8; ++q) y[q] += (float)r[q];
     }
@@ -628,6 +670,21 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
     SCN_MX_MULTIPLY(0, 0, y)
   }
   SCN_MX_MULTIPLY(1, 2, y)
+  // what this lane will store, and the fp16 residual it needs there, fetched while the last stage travels (the kernel whose
+  // accumulators leave registers for it)
+  constexpr int LPR = 4 * TN, RPP = 64 / LPR, PASSES = 32 / RPP;   // lanes per row (8 channels each), rows per pass
+  constexpr bool PRE = TN * TM <= 4;
+  const uint32_t row0 = i0 + wm * 32 * TM + lane / LPR, ch = n0 + wn * 32 * TN + (lane % LPR) * 8;
+  v4u pre[PRE ? TM * PASSES : 1];
+  if constexpr (PRE) {
+    const bool want = p.res && !p.res_fp32 && ch + 8 <= p.n;
+#pragma unroll
+    for (int q = 0; q < TM * PASSES; ++q) {
+      pre[q] = v4u{0, 0, 0, 0};
+      const uint32_t row = row0 + q * RPP;
+      if (want && row < m) __builtin_memcpy(&pre[q], (const _Float16*)p.res + (size_t)row * p.res_ld + ch, 16);
+    }
+  }
   {   // the last stage, of 1 .. 8 blocks
     SCN_MX_BARRIER()
     const uint32_t left = p.kb - st * 8;
@@ -655,7 +712,6 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
   // Store through LDS (wave-private, 32 rows at a time): a lane of the accumulators holds 4 consecutive channels of one
   // row, a store wants whole 128-byte lines of a row.
   float* buf = reinterpret_cast<float*>(lds) + wave * 32 * T::PAD;
-  constexpr int LPR = 4 * TN, RPP = 64 / LPR;   // lanes per row (8 channels each), rows per pass
 #pragma unroll
   for (int b = 0; b < TM; ++b) {
 #pragma unroll
@@ -664,10 +720,12 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
       for (int q = 0; q < 4; ++q)
         *reinterpret_cast<v4f*>(buf + ln * T::PAD + a * 32 + q * 8 + lh * 4) =
             v4f{acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]};
-    const uint32_t row0 = i0 + wm * 32 * TM + b * 32, ch = n0 + wn * 32 * TN + (lane % LPR) * 8;
-#pragma unroll 2
-    for (int r = lane / LPR; r < 32; r += RPP)
-      if (row0 + r < m && ch < p.n) product_store8(p, row0 + r, ch, buf + r * T::PAD + (lane % LPR) * 8);
+#pragma unroll
+    for (int r = 0; r < PASSES; ++r) {
+      const uint32_t row = row0 + (b * PASSES + r) * RPP;
+      if (row < m && ch < p.n)
+        product_store8<PRE>(p, row, ch, buf + (r * RPP + lane / LPR) * T::PAD + (lane % LPR) * 8, pre[PRE ? b * PASSES + r : 0]);
+    }
   }
 }
 
@@ -684,9 +742,22 @@ static int launch_product(const ProductArgs& p, hipStream_t stream) {
   return SCN_OK;
 }
 
-constexpr uint32_t kDirectRows = 16;
+// Rows that are not quantised yet are quantised by every workgroup that reads them up to this many blocks; beyond it (and
+// beyond 16 rows) a launch of its own is cheaper: 8192 x 8192 weights, 4 fp16 rows (1024 blocks): 15.4 us against 15.8 us,
+// 8 rows 19.9 us against 17.3 us.
+static bool product_direct(uint32_t m, uint32_t k) { return m <= 16 && (uint64_t)m * mx_blocks(k) <= kFewBlocks; }
+static size_t product_workspace(uint32_t m, uint32_t k) { return product_direct(m, k) ? 0 : (size_t)m * mx_row_bytes(k); }
 
-static size_t product_workspace(uint32_t m, uint32_t k) { return (size_t)m * mx_row_bytes(k); }
+// U = runs a wave requests at once: what it has to do in all, up to 8 (4 for two row tiles).
+template <int AT, int MT>
+static void launch_few(const ProductArgs& p, hipStream_t stream) {
+  const uint32_t runs = (p.kb + 3) / 4, waves = std::min(8u, runs), per = ceil_div(runs, waves);
+  const dim3 grid(ceil_div(p.n, 16)), block(64 * waves);
+  if (per == 1) hipLaunchKernelGGL((k_mx_product_few<AT, MT, 1>), grid, block, 0, stream, p);
+  else if (per == 2) hipLaunchKernelGGL((k_mx_product_few<AT, MT, 2>), grid, block, 0, stream, p);
+  else if (per <= 4 || MT > 1) hipLaunchKernelGGL((k_mx_product_few<AT, MT, 4>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((k_mx_product_few<AT, 1, 8>), grid, block, 0, stream, p);
+}
 
 int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
   SCN_REQUIRE(io.a_dtype == SCN_DTYPE_MXFP4 || io.a_dtype == SCN_DTYPE_FP16 || io.a_dtype == SCN_DTYPE_FP32, SCN_ERR_INVALID,
@@ -737,7 +808,7 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
   } else {
     SCN_REQUIRE(io.a_dev && aligned(io.a_dev, at) && io.a_ld >= io.k, SCN_ERR_INVALID,
                 "mx_product: null or misaligned rows, or row stride %u < %u channels", io.a_ld, io.k);
-    if (io.m > kDirectRows) {
+    if (!product_direct(io.m, io.k)) {
       const size_t need = product_workspace(io.m, io.k);
       SCN_REQUIRE(io.workspace_dev && ((uintptr_t)io.workspace_dev & 15) == 0 && io.workspace_bytes >= need, SCN_ERR_INVALID,
                   "mx_product: rows of this type need a 16-byte aligned workspace of %zu bytes (%zu given)", need, io.workspace_bytes);
@@ -751,12 +822,13 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
       at = SCN_DTYPE_MXFP4;
     }
   }
-  if (io.m <= kDirectRows) {
-    const dim3 grid(ceil_div(io.n, 16));
-    if (at == SCN_DTYPE_MXFP4) hipLaunchKernelGGL(k_mx_product_few<SCN_DTYPE_MXFP4>, grid, dim3(512), 0, stream, p);
-    else if (at == SCN_DTYPE_FP16) hipLaunchKernelGGL(k_mx_product_few<SCN_DTYPE_FP16>, grid, dim3(512), 0, stream, p);
-    else hipLaunchKernelGGL(k_mx_product_few<SCN_DTYPE_FP32>, grid, dim3(512), 0, stream, p);
-  } else {
+  if (at == SCN_DTYPE_FP16) launch_few<SCN_DTYPE_FP16, 1>(p, stream);
+  else if (at == SCN_DTYPE_FP32) launch_few<SCN_DTYPE_FP32, 1>(p, stream);
+  else if (io.m <= 16) launch_few<SCN_DTYPE_MXFP4, 1>(p, stream);
+  // two row tiles of 16 where the tiled kernel below would run few workgroups down a long k: 32 rows, 1024 x 1024 weights 3.5
+  // against 4.0 us, 4096 x 16384 24.5 against 36.6; but 8192 x 8192 24.6 against 20.3, 256 x 128 4.1 against 3.1
+  else if (io.m <= 32 && kb >= 32 && io.n <= 4096) launch_few<SCN_DTYPE_MXFP4, 2>(p, stream);
+  else {
     // the largest tile of which there are enough for the GPU's 256 CUs
     const uint64_t t256 = (uint64_t)ceil_div(io.n, 256) * ceil_div(io.m, 256), t128 = (uint64_t)ceil_div(io.n, 128) * ceil_div(io.m, 128);
     int rc = t256 >= 256 && kb > 8 ? launch_product<256, 256, 4, 2>(p, stream)
@@ -794,8 +866,7 @@ int scn_mx_dequantize_rows(const uint8_t* codes_dev, uint32_t codes_ld, const ui
   return rc;
 }
 
-uint32_t scn_mx_product_direct_rows(void) { return kDirectRows; }
-size_t scn_mx_product_workspace(uint32_t m, uint32_t k) { return m > kDirectRows ? product_workspace(m, k) : 0; }
+size_t scn_mx_product_workspace(uint32_t m, uint32_t k) { return k ? product_workspace(m, k) : 0; }
 
 int scn_mx_product(const scn_mx_product_io* io, void* stream) {
   SCN_REQUIRE(io, SCN_ERR_INVALID, "scn_mx_product: null pointer");
