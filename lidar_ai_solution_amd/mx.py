@@ -10,7 +10,6 @@ rows" in scn_c_api.h for the format).  PyTorch only owns memory and streams; the
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import struct
 from typing import Optional, Sequence
@@ -23,7 +22,7 @@ from .scn import _stream_ptr
 
 _DTYPE = {torch.float16: capi.DTYPE_FP16, torch.float32: capi.DTYPE_FP32, torch.int8: capi.DTYPE_INT8}
 _FLOATS = (torch.float16, torch.float32)
-_HERE = contextlib.nullcontext()
+_ROWS = (torch.float16, torch.float32, torch.int8)
 _L = None
 
 
@@ -34,18 +33,22 @@ def _lib():
     return _L
 
 
-def _on(index: int):
-    """The rows' device as the current one (these calls take a few microseconds: no context is entered without need)."""
-    return _HERE if torch.cuda.current_device() == index else torch.cuda.device(index)
+_current_device = torch.cuda.current_device   # (a call here takes a few microseconds: a device context is entered only where needed)
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # (a tenth of the time of building a Stream object)
 
 
-def _stream(stream, index: int):
-    if stream is not None:
-        return _stream_ptr(stream)
+def _stream(index: int) -> int:
     return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _using(stream, index: int):
+    """A context in which `stream` (a torch stream or a hipStream_t) is the current one: what a call allocates then belongs
+    to the stream that its kernels run on."""
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(int(stream), device=index) if int(stream) else torch.cuda.default_stream(index)
+    return torch.cuda.stream(stream)
 
 
 def row_bytes(channels: int) -> int:
@@ -81,26 +84,30 @@ class MxRows:
         if channels < 1 or n < 0:
             raise ValueError("rows need at least one channel")
         self = cls.__new__(cls)
-        size = row_bytes(channels)
-        buf = torch.empty((n, size), dtype=torch.uint8, device=device)
+        blocks = (channels + 31) // 32
+        size = (16 * blocks + (blocks + 3) // 4 * 4 + 15) // 16 * 16      # row_bytes(channels)
+        buf = torch.empty(n * size, dtype=torch.uint8, device=device)     # (flat: made in two thirds of the time)
         self._codes = self._scales = None
-        self._buffer, self.channels, self.num_rows, self.index = buf, int(channels), int(n), buf.get_device()
-        self.codes_ptr = buf.data_ptr()
-        self.scales_ptr = self.codes_ptr + 16 * ((channels + 31) // 32)
+        self._buffer, self.channels, self.num_rows, self.index = buf, channels, n, buf.get_device()
+        self.codes_ptr = ptr = buf.data_ptr()
+        self.scales_ptr = ptr + 16 * blocks
         self.codes_ld = self.scales_ld = size
         return self
+
+    def _columns(self, first: int, last: int) -> torch.Tensor:
+        return self._buffer.view(self.num_rows, self.codes_ld)[:, first:last]
 
     @property
     def codes(self) -> torch.Tensor:
         if self._codes is None:
-            self._codes = self._buffer[:, :16 * ((self.channels + 31) // 32)]
+            self._codes = self._columns(0, 16 * ((self.channels + 31) // 32))
         return self._codes
 
     @property
     def scales(self) -> torch.Tensor:
         if self._scales is None:
             blocks = (self.channels + 31) // 32
-            self._scales = self._buffer[:, 16 * blocks:16 * blocks + (blocks + 3) // 4 * 4]
+            self._scales = self._columns(16 * blocks, 16 * blocks + (blocks + 3) // 4 * 4)
         return self._scales
 
     @property
@@ -143,16 +150,22 @@ def quantize_rows(x: torch.Tensor, relu: bool = False, dynamic_range: float = 0.
                   out: Optional[MxRows] = None, stream=None) -> MxRows:
     """x: fp16, fp32 or int8 (value = q * dynamic_range / 127) rows [n, c]; num: device-side row count (rows beyond it are
     left as they were)."""
-    ld = _check_rows(x, (torch.float16, torch.float32, torch.int8), "x")
+    ld = _check_rows(x, _ROWS, "x")
     n, c = x.shape
     index = x.get_device()
-    with _on(index):
-        if out is None:
-            out = MxRows.empty(n, c, x.device)
-        elif out.num_rows < n or out.channels != c or out.index != index:
-            raise ValueError("out does not fit x")
-        rc = _lib().scn_mx_quantize_rows(x.data_ptr(), _DTYPE[x.dtype], c, ld, dynamic_range, relu, out.codes_ptr, out.codes_ld,
-                                         out.scales_ptr, out.scales_ld, n, _count_ptr(num, index), _stream(stream, index))
+    if stream is not None:
+        with _using(stream, index):
+            return quantize_rows(x, relu, dynamic_range, num, out)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return quantize_rows(x, relu, dynamic_range, num, out)
+    if out is None:
+        out = MxRows.empty(n, c, x.device)
+    elif out.num_rows < n or out.channels != c or out.index != index:
+        raise ValueError("out does not fit x")
+    rc = _lib().scn_mx_quantize_rows(x.data_ptr(), _DTYPE[x.dtype], c, ld, dynamic_range, relu, out.codes_ptr, out.codes_ld,
+                                     out.scales_ptr, out.scales_ld, n, None if num is None else _count_ptr(num, index),
+                                     _stream(index))
     if rc:
         capi.check(rc)
     return out
@@ -161,18 +174,24 @@ def quantize_rows(x: torch.Tensor, relu: bool = False, dynamic_range: float = 0.
 def dequantize_rows(rows: MxRows, dtype: torch.dtype = torch.float16, num: Optional[torch.Tensor] = None,
                     out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     n, c, index = rows.num_rows, rows.channels, rows.index
-    with _on(index):
-        if out is None:
-            if dtype not in _FLOATS:
-                raise ValueError("dtype must be float16 or float32")
-            out, ld = torch.empty((n, c), dtype=dtype, device="cuda"), c
-        else:
-            ld = _check_rows(out, _FLOATS, "out")
-            if out.shape[0] < n or out.shape[1] != c:
-                raise ValueError("out does not fit the rows")
-            _same_device(index, out)
-        rc = _lib().scn_mx_dequantize_rows(rows.codes_ptr, rows.codes_ld, rows.scales_ptr, rows.scales_ld, c, out.data_ptr(),
-                                           _DTYPE[out.dtype], ld, n, _count_ptr(num, index), _stream(stream, index))
+    if stream is not None:
+        with _using(stream, index):
+            return dequantize_rows(rows, dtype, num, out)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return dequantize_rows(rows, dtype, num, out)
+    if out is None:
+        if dtype not in _FLOATS:
+            raise ValueError("dtype must be float16 or float32")
+        out, ld = torch.empty((n, c), dtype=dtype, device="cuda"), c
+    else:
+        ld = _check_rows(out, _FLOATS, "out")
+        if out.shape[0] < n or out.shape[1] != c:
+            raise ValueError("out does not fit the rows")
+        _same_device(index, out)
+    rc = _lib().scn_mx_dequantize_rows(rows.codes_ptr, rows.codes_ld, rows.scales_ptr, rows.scales_ld, c, out.data_ptr(),
+                                       _DTYPE[out.dtype], ld, n, None if num is None else _count_ptr(num, index),
+                                       _stream(index))
     if rc:
         capi.check(rc)
     return out
@@ -191,53 +210,58 @@ def product(a, b: MxRows, bias: Optional[torch.Tensor] = None, relu: bool = Fals
     given); calls that may overlap need one each."""
     L = _lib()
     n, index = b.num_rows, b.index
-    with _on(index):
-        ws_ptr = ws_bytes = 0
-        if isinstance(a, MxRows):
-            m, k, a_index = a.num_rows, a.channels, a.index
-            a_ptr, a_dtype, a_ld, as_ptr, as_ld = a.codes_ptr, capi.DTYPE_MXFP4, a.codes_ld, a.scales_ptr, a.scales_ld
-        else:
-            a_ld = _check_rows(a, _FLOATS, "a")
-            (m, k), a_index = a.shape, a.get_device()
-            a_ptr, a_dtype, as_ptr, as_ld = a.data_ptr(), _DTYPE[a.dtype], 0, 0
-            if workspace is None:
-                ws_bytes = L.scn_mx_product_workspace(m, k)
-                if ws_bytes:
-                    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device="cuda")
-            if workspace is not None:
-                if not workspace.is_contiguous():
-                    raise ValueError("workspace must be contiguous")
-                _same_device(index, workspace)
-                ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        if a_index != index:
-            raise ValueError(f"rows on cuda:{a_index}, weights on cuda:{index}")
-        if b.channels != k:
-            raise ValueError(f"rows of {k} channels times weights of {b.channels}")
-        if out is None:
-            if out_dtype not in _FLOATS:
-                raise ValueError("out_dtype must be float16 or float32")
-            out, out_ld = torch.empty((m, n), dtype=out_dtype, device="cuda"), n
-        else:
-            out_ld = _check_rows(out, _FLOATS, "out")
-            if out.shape[0] < m or out.shape[1] != n:
-                raise ValueError("out does not fit the product")
-            _same_device(index, out)
-        bias_ptr = bias_dtype = res_ptr = res_dtype = res_ld = 0
-        if bias is not None:
-            if bias.dtype not in _FLOATS or bias.shape != (n,) or not bias.is_contiguous():
-                raise ValueError(f"bias must be {n} contiguous fp16 or fp32 values")
-            _same_device(index, bias)
-            bias_ptr, bias_dtype = bias.data_ptr(), _DTYPE[bias.dtype]
-        if residual is not None:
-            res_ld = _check_rows(residual, _FLOATS, "residual")
-            if residual.shape[0] < m or residual.shape[1] != n:
-                raise ValueError("residual does not fit the product")
-            _same_device(index, residual)
-            res_ptr, res_dtype = residual.data_ptr(), _DTYPE[residual.dtype]
-        rc = L.scn_mx_product(_PRODUCT_IO.pack(a_ptr, a_dtype, a_ld, as_ptr, as_ld, b.codes_ptr, b.codes_ld, b.scales_ptr, b.scales_ld,
-                                               m, n, k, _count_ptr(num, index) or 0, bias_ptr, bias_dtype, bool(relu), res_ptr,
-                                               res_dtype, res_ld, bool(relu_after_add), out.data_ptr(), _DTYPE[out.dtype], out_ld,
-                                               ws_ptr, ws_bytes), _stream(stream, index))
+    if stream is not None:
+        with _using(stream, index):
+            return product(a, b, bias, relu, residual, relu_after_add, out_dtype, num, out, workspace)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return product(a, b, bias, relu, residual, relu_after_add, out_dtype, num, out, workspace)
+    ws_ptr = ws_bytes = 0
+    if isinstance(a, MxRows):
+        m, k, a_index = a.num_rows, a.channels, a.index
+        a_ptr, a_dtype, a_ld, as_ptr, as_ld = a.codes_ptr, capi.DTYPE_MXFP4, a.codes_ld, a.scales_ptr, a.scales_ld
+    else:
+        a_ld = _check_rows(a, _FLOATS, "a")
+        (m, k), a_index = a.shape, a.get_device()
+        a_ptr, a_dtype, as_ptr, as_ld = a.data_ptr(), _DTYPE[a.dtype], 0, 0
+        if workspace is None:
+            ws_bytes = L.scn_mx_product_workspace(m, k)
+            if ws_bytes:
+                workspace = torch.empty(ws_bytes, dtype=torch.uint8, device="cuda")
+        if workspace is not None:
+            if not workspace.is_contiguous():
+                raise ValueError("workspace must be contiguous")
+            _same_device(index, workspace)
+            ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    if a_index != index:
+        raise ValueError(f"rows on cuda:{a_index}, weights on cuda:{index}")
+    if b.channels != k:
+        raise ValueError(f"rows of {k} channels times weights of {b.channels}")
+    if out is None:
+        if out_dtype not in _FLOATS:
+            raise ValueError("out_dtype must be float16 or float32")
+        out, out_ld = torch.empty((m, n), dtype=out_dtype, device="cuda"), n
+    else:
+        out_ld = _check_rows(out, _FLOATS, "out")
+        if out.shape[0] < m or out.shape[1] != n:
+            raise ValueError("out does not fit the product")
+        _same_device(index, out)
+    bias_ptr = bias_dtype = res_ptr = res_dtype = res_ld = 0
+    if bias is not None:
+        if bias.dtype not in _FLOATS or bias.shape != (n,) or not bias.is_contiguous():
+            raise ValueError(f"bias must be {n} contiguous fp16 or fp32 values")
+        _same_device(index, bias)
+        bias_ptr, bias_dtype = bias.data_ptr(), _DTYPE[bias.dtype]
+    if residual is not None:
+        res_ld = _check_rows(residual, _FLOATS, "residual")
+        if residual.shape[0] < m or residual.shape[1] != n:
+            raise ValueError("residual does not fit the product")
+        _same_device(index, residual)
+        res_ptr, res_dtype = residual.data_ptr(), _DTYPE[residual.dtype]
+    rc = L.scn_mx_product(_PRODUCT_IO.pack(a_ptr, a_dtype, a_ld, as_ptr, as_ld, b.codes_ptr, b.codes_ld, b.scales_ptr, b.scales_ld,
+                                           m, n, k, 0 if num is None else _count_ptr(num, index), bias_ptr, bias_dtype, bool(relu), res_ptr,
+                                           res_dtype, res_ld, bool(relu_after_add), out.data_ptr(), _DTYPE[out.dtype], out_ld,
+                                           ws_ptr, ws_bytes), _stream(index))
     if rc:
         capi.check(rc)
     return out
@@ -316,25 +340,30 @@ class Conv:
         if x.codes_ld != x.scales_ld or x.scales_ptr != x.codes_ptr + 16 * blocks:
             raise ValueError("the convolution reads rows in the one-buffer form (codes, then scales)")
         wide = (self.cout + 15) // 16 * 16
-        with _on(x.index):
-            if out is None:
-                out, out_ld = torch.empty((max_rows, wide), dtype=torch.float16, device="cuda"), wide
-            else:
-                out_ld = _check_rows(out, (torch.float16,), "out")
-                if out.shape[0] < max_rows or out.shape[1] < wide:
-                    raise ValueError(f"out must hold {max_rows} rows of {wide} channels")
-                _same_device(x.index, out)
-            io = capi.ConvIO()
-            io.x_dev, io.x_ld = x.codes_ptr, x.codes_ld
-            io.relu, io.out_dtype, io.out_dev, io.out_ld = int(bool(relu)), capi.DTYPE_FP16, out.data_ptr(), out_ld
-            if residual is not None:
-                io.res_ld = _check_rows(residual, (torch.float16,), "residual")
-                if residual.shape[0] < max_rows or residual.shape[1] < wide:
-                    raise ValueError(f"residual must hold {max_rows} rows of {wide} channels")
-                _same_device(x.index, residual)
-                io.res_dev, io.res_dtype, io.mid_dtype = residual.data_ptr(), capi.DTYPE_FP16, capi.DTYPE_FP16
-                io.relu_after_add = int(bool(relu_after_add))
-            capi.check(_lib().scn_conv_forward(self._h, rulebook._h, C.byref(io), _stream(stream, x.index)))
+        if stream is not None:
+            with _using(stream, x.index):
+                return self.forward(x, rulebook, max_rows, relu, residual, relu_after_add, out)
+        if x.index != _current_device():
+            with torch.cuda.device(x.index):
+                return self.forward(x, rulebook, max_rows, relu, residual, relu_after_add, out)
+        if out is None:
+            out, out_ld = torch.empty((max_rows, wide), dtype=torch.float16, device="cuda"), wide
+        else:
+            out_ld = _check_rows(out, (torch.float16,), "out")
+            if out.shape[0] < max_rows or out.shape[1] < wide:
+                raise ValueError(f"out must hold {max_rows} rows of {wide} channels")
+            _same_device(x.index, out)
+        io = capi.ConvIO()
+        io.x_dev, io.x_ld = x.codes_ptr, x.codes_ld
+        io.relu, io.out_dtype, io.out_dev, io.out_ld = int(bool(relu)), capi.DTYPE_FP16, out.data_ptr(), out_ld
+        if residual is not None:
+            io.res_ld = _check_rows(residual, (torch.float16,), "residual")
+            if residual.shape[0] < max_rows or residual.shape[1] < wide:
+                raise ValueError(f"residual must hold {max_rows} rows of {wide} channels")
+            _same_device(x.index, residual)
+            io.res_dev, io.res_dtype, io.mid_dtype = residual.data_ptr(), capi.DTYPE_FP16, capi.DTYPE_FP16
+            io.relu_after_add = int(bool(relu_after_add))
+        capi.check(_lib().scn_conv_forward(self._h, rulebook._h, C.byref(io), _stream(x.index)))
         if out.shape == (max_rows, self.cout):
             return out
         return out[:max_rows, :self.cout]

@@ -292,6 +292,29 @@ def test_product_is_the_same_every_time_and_on_another_stream():
         assert torch.equal(first, second)
 
 
+def test_calls_on_a_stream_of_their_own_own_their_memory():
+    """Buffers that a call allocates belong to the stream it was given: work on the current stream does not get them while the
+    other stream still uses them."""
+    mx = _mx()
+    rng = np.random.default_rng(12)
+    w, wv = mx_rows(rng, 256, 512)
+    h = rows(rng, 3000, 512)
+    x = torch.from_numpy(h).to(DEV)
+    y, mag = R.product(R.fake(h), wv)
+    side = torch.cuda.Stream()
+    for stream in (side, side.cuda_stream):
+        torch.cuda.synchronize()
+        got = []
+        for _ in range(4):
+            got.append(mx.dequantize_rows(mx.quantize_rows(mx.product(x, w, stream=stream), stream=stream), torch.float32, stream=stream))
+            junk = [torch.full((3000, 256), 7.0, dtype=torch.float16, device=DEV) for _ in range(3)]   # wants freed memory
+        torch.cuda.synchronize()
+        first = mx.product(x, w)
+        R.within(first.double().cpu().numpy(), y, R.tolerance(y, mag, 512, 2.0 ** -11))
+        want = mx.dequantize_rows(mx.quantize_rows(first), torch.float32)
+        assert all(torch.equal(g.view(torch.int32), want.view(torch.int32)) for g in got) and len(junk) == 3   # (bits: infinite products quantise to NaN)
+
+
 # ------------------------------------------------------------------------------------------------- convolution
 def scene(rng, n, grid):
     cells = np.sort(rng.choice(grid[0] * grid[1] * grid[2], n, replace=False))
