@@ -96,26 +96,26 @@ bool ConvWeights::init(const uint16_t* w_fp16, const int shape[5], const float* 
   return true;
 }
 
-// Weights of a convolution on microscaled rows, in the operand order of the 32x32 scaled matrix instruction: lane l of
-// fragment (step s, tile t) is output channel 32 t + l % 32, block 2 s + l / 32 of the sequence (offset, block of the row).
+// Weights of a convolution on microscaled rows: block g (kernel offset, block of the row) of the 32 output channels of a
+// tile is one unit of 32 x 16 code bytes, wfrag[g][tile][channel]; their scale bytes wscale[g][tile][channel].
 bool ConvWeights::init_mx(const uint16_t* w_fp16, const uint16_t* bias_fp16) {
-  std::vector<uint8_t> frag((size_t)steps * mtiles32 * 64 * 16, 0), sc((size_t)steps * mtiles32 * 64, 0);
-  std::vector<float> bs((size_t)mtiles32 * 32, 0.f);
+  const int tiles = (cout + 31) / 32;
+  const size_t units = (size_t)kvol * chunks * tiles;
+  std::vector<uint8_t> frag(units * 32 * 16, 0), sc(units * 32, 0);
+  std::vector<float> bs((size_t)tiles * 32, 0.f);
   if (bias_fp16)
     for (int c = 0; c < cout; ++c) bs[c] = half_bits_to_float(bias_fp16[c]);
   float v[32];
-  for (int s = 0; s < steps; ++s)
-    for (int t = 0; t < mtiles32; ++t)
-      for (int l = 0; l < 64; ++l) {
-        const int g = 2 * s + l / 32, k = g / chunks, b = g % chunks, co = 32 * t + l % 32;
-        if (k >= kvol || co >= cout) continue;
-        const int nv = cin - 32 * b < 32 ? cin - 32 * b : 32;
-        for (int i = 0; i < nv; ++i) v[i] = half_bits_to_float(w_fp16[((size_t)co * kvol + k) * cin + 32 * b + i]);
-        const size_t f = ((size_t)s * mtiles32 + t) * 64 + l;
-        sc[f] = mx_quantize_block(v, nv, &frag[f * 16]);
-      }
-  if (!wfrag.alloc(frag.size()) || !wscale.alloc(sc.size()) || !bias.alloc(bs.size() * 4)) return false;
-  if (hipMemcpy(wfrag.p, frag.data(), frag.size(), hipMemcpyHostToDevice) != hipSuccess ||
+  for (int g = 0; g < kvol * chunks; ++g)
+    for (int co = 0; co < cout; ++co) {
+      const int k = g / chunks, b = g % chunks, nv = std::min(32, cin - 32 * b);
+      for (int i = 0; i < nv; ++i) v[i] = half_bits_to_float(w_fp16[((size_t)co * kvol + k) * cin + 32 * b + i]);
+      const size_t f = ((size_t)g * tiles + co / 32) * 32 + co % 32;
+      sc[f] = mx_quantize_block(v, nv, &frag[f * 16]);
+    }
+  if (!zrow.alloc(1536) || !wfrag.alloc(frag.size()) || !wscale.alloc(sc.size()) || !bias.alloc(bs.size() * 4)) return false;
+  if (hipMemset(zrow.p, 0, 512) != hipSuccess || hipMemset(zrow.as<char>() + 512, 0xFF, 1024) != hipSuccess ||
+      hipMemcpy(wfrag.p, frag.data(), frag.size(), hipMemcpyHostToDevice) != hipSuccess ||
       hipMemcpy(wscale.p, sc.data(), sc.size(), hipMemcpyHostToDevice) != hipSuccess ||
       hipMemcpy(bias.p, bs.data(), bs.size() * 4, hipMemcpyHostToDevice) != hipSuccess) {
     set_error("weight upload failed");

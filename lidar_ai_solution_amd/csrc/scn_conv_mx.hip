@@ -7,10 +7,16 @@ namespace scn {
 typedef int v8i __attribute__((ext_vector_type(8)));
 
 // v_mfma_scale_f32_32x32x64_f8f6f4 with 4-bit operands: lane l supplies row / column l % 32, the 16 code bytes of K-block
-// l / 32 and that block's scale.  K-step s consumes blocks 2s and 2s + 1 of the sequence (offset 0 block 0, offset 0
-// block 1, ..., offset kvol-1 block BPR-1), BPR = blocks of an input row: a lane gathers 16 contiguous code bytes and one
-// scale byte of one input row.
-//   MT = tiles of 32 output channels a wave owns; wider layers take more workgroups (grid y)
+// l / 32 and that block's scale.  Rows of A are output channels, columns of B voxels (as in the other convolution kernels); a
+// K-step takes two blocks.  Weights are laid out in units of one block x 32 output channels: wfrag[block][tile][32] x 16
+// bytes, scale bytes wscales[block][tile][32]; block g = kernel offset * BPR + block of the row (BPR = blocks of an input row).
+__device__ __forceinline__ v16f conv_mma(const uint4& w, uint32_t ws, const uint4& x, uint32_t xs, v16f c) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v8i{(int)w.x, (int)w.y, (int)w.z, (int)w.w, 0, 0, 0, 0},
+                                                         v8i{(int)x.x, (int)x.y, (int)x.z, (int)x.w, 0, 0, 0, 0}, c, 4, 4, 0,
+                                                         (int)ws, 0, (int)xs);
+}
+
+// Any width: operands straight from memory, a wave owns 32 rows x MT tiles of 32 output channels.
 template <int MT>
 __global__ __launch_bounds__(256) void k_conv_mx_rows(const ConvArgs a, const uint8_t* __restrict__ wscales, int bpr, int mtiles) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -35,20 +41,16 @@ __global__ __launch_bounds__(256) void k_conv_mx_rows(const ConvArgs a, const ui
     if (g < total && row < n) idx = a.nbr[(size_t)k * a.nbr_ld + row];
     if (!__any(idx >= 0)) continue;   // no row of this wave has a neighbour at these blocks
     uint4 xq = make_uint4(0, 0, 0, 0);
-    int xs = 0;
+    uint32_t xs = 0;
     if (idx >= 0) {
       const char* src = a.x + (size_t)(uint32_t)idx * a.x_ld_bytes;
       xq = *reinterpret_cast<const uint4*>(src + b * 16);
       xs = *reinterpret_cast<const uint8_t*>(src + bpr * 16 + b);
     }
-    const v8i xv = {(int)xq.x, (int)xq.y, (int)xq.z, (int)xq.w, 0, 0, 0, 0};
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      const size_t f = ((size_t)s * mtiles + min(t0 + t, mtiles - 1)) * 64 + lane;
-      const uint4 wq = a.wfrag[f];
-      const int ws = wscales[f];
-      const v8i wv = {(int)wq.x, (int)wq.y, (int)wq.z, (int)wq.w, 0, 0, 0, 0};
-      acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv, xv, acc[t], 4, 4, 0, ws, 0, xs);
+      const size_t f = ((size_t)min(g, total - 1) * mtiles + min(t0 + t, mtiles - 1)) * 32 + ln;
+      acc[t] = conv_mma(a.wfrag[f], wscales[f], xq, xs, acc[t]);
     }
   }
   if (row >= n) return;
@@ -64,11 +66,286 @@ __global__ __launch_bounds__(256) void k_conv_mx_rows(const ConvArgs a, const ui
     }
 }
 
+// Rows of up to 4 blocks (128 channels).  What bounds the kernel above is the memory pipe: 16 code bytes of 32 rows in operand
+// order are 32 requests, their scale bytes 32 more.  Here a row is fetched whole -- codes and the scale word behind them are
+// BPR + 1 chunks of 16 bytes, taken by as many neighbouring lanes -- straight into LDS, and the operands are read from there.
+// A workgroup owns 64 rows and MT tiles of 32 output channels; its W waves share the rows' neighbour indices and deal the
+// kernel offsets out between them, so a wave only ever waits for its own loads; the waves' sums are added (in wave order) when
+// the rows are stored.
+//   a stage = one kernel offset that some row has a neighbour at (two of them for rows of one block): 64 gathered rows and
+//   the weights of its blocks; a wave fetches one stage ahead (two ahead leave room for fewer waves: 120,000 rows 64 -> 64
+//   36.6 against 23.8 us).  Rows without a neighbour fetch zeros (scale 2^-127, codes 0).
+//   LDS rows of 3 and 5 chunks are read without bank conflicts as they are; rows of 2 and 4 chunks hold chunk c at position
+//   c ^ (row / 8) % 2 and c ^ (row / 4) % 4.
+template <int BPR, int MT, int W>
+struct ConvMxStage {
+  static constexpr int OFFS = BPR == 1 ? 2 : 1;                  // kernel offsets of a stage
+  static constexpr int SB = BPR * OFFS, KS = (SB + 1) / 2;       // blocks and K-steps
+  static constexpr int CH = BPR + 1;                             // 16-byte chunks of a row
+  static constexpr int GLOADS = CH * OFFS;                       // wave loads: 64 rows
+  static constexpr int WLOADS = (SB * MT + 1) / 2, SLOADS = (SB * MT + 7) / 8;   // weight units of 512 bytes, their scales
+  static constexpr int LOADS = GLOADS + WLOADS + SLOADS;
+  static constexpr int WOFF = GLOADS * 1024, SOFF = WOFF + WLOADS * 1024, BYTES = SOFF + SLOADS * 256;
+  static constexpr int KMAX = 27;                                // kernel offsets whose indices are held at a time
+  static constexpr int RING = KMAX * 256;                        // LDS offset of the rings
+  static constexpr int PAD = 32 * MT + 4;                        // floats per row of the store buffer
+  static constexpr int WAVE = 2 * BYTES > 32 * PAD * 4 ? 2 * BYTES : 32 * PAD * 4;
+  static constexpr int LDS = RING + W * WAVE;
+};
+
+// 64 x 16 (or 64 x 4) bytes to LDS, lane l's to base + 16 l (4 l): in assembly, because the compiler would order its own LDS
+// reads behind every such load in flight.  m0 has no other user in this kernel.
+__device__ __forceinline__ void conv_load16_lds(const void* src, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(base) : "memory");
+}
+// (a wave's base and a 32-bit offset per lane)
+__device__ __forceinline__ void conv_load16_lds(const void* src, uint32_t offset, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(src), "s"(base) : "memory");
+}
+__device__ __forceinline__ void conv_load4_lds(const void* src, uint32_t offset, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(src), "s"(base) : "memory");
+}
+__device__ __forceinline__ void conv_load4_lds(const void* src, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(base) : "memory");
+}
+
+// MODE: the epilogue (see epilogue_values): 2 and 4 are fp16 output without and with an fp16 residual, 0 everything.
+template <int BPR, int MT, int W, int MODE>
+__global__ __launch_bounds__(64 * W, 2) void k_conv_mx_gather(const ConvArgs a, const uint8_t* __restrict__ wscales, int mtiles) {
+  using S = ConvMxStage<BPR, MT, W>;
+  __shared__ __align__(16) char lds[S::LDS];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = lane & 31, lh = lane >> 5;
+  const uint32_t n = eff_n(a.n_out_dev, a.n_bound);
+  uint32_t tile;
+  if (!xcd_tile(n, 64u, &tile)) return;
+  const uint32_t row0 = tile * 64;
+  const int t0 = blockIdx.y * MT;
+  typedef __attribute__((address_space(3))) char* lptr;
+  const uint32_t base = (uint32_t)(uintptr_t)(lptr)lds;
+  const int32_t* idx = reinterpret_cast<const int32_t*>(lds);
+  const int ring = S::RING + wave * S::WAVE;
+
+  v16f acc[MT][2];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[t][u][j] = 0.f;
+
+  // what this lane fetches of a stage: for gather load q (of one offset) the row and the chunk, for the weight and scale loads
+  // the unit (block and tile) counted from the offset's first block
+  int grow[S::CH], gchunk[S::CH];
+#pragma unroll
+  for (int q = 0; q < S::CH; ++q) {
+    const int e = q * 64 + lane, r = e / S::CH, p = e - r * S::CH;
+    grow[q] = r;
+    gchunk[q] = (S::CH == 2 ? p ^ ((r >> 3) & 1) : S::CH == 4 ? p ^ ((r >> 2) & 3) : p) * 16;
+  }
+  auto unit_of = [&](int u) {
+    u = min(u, S::SB * MT - 1);
+    const int b = u / MT, t = u - b * MT;
+    return (uint32_t)((BPR == 1 ? 0 : b) * mtiles + min(t0 + t, mtiles - 1));
+  };
+  uint32_t wunit[S::WLOADS], sunit[S::SLOADS];
+#pragma unroll
+  for (int q = 0; q < S::WLOADS; ++q) wunit[q] = unit_of(2 * q + lh);
+#pragma unroll
+  for (int q = 0; q < S::SLOADS; ++q) sunit[q] = unit_of(8 * q + lane / 8);
+
+  for (int k0 = 0; k0 < a.kvol; k0 += S::KMAX) {
+    // neighbour rows of up to KMAX offsets; rows beyond the count have none
+    const int nk = min(S::KMAX, a.kvol - k0);
+    const int32_t* minus1 = reinterpret_cast<const int32_t*>(a.zrow + 512);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (W > 1 && k0) __syncthreads();   // (the indices before these have been read)
+    for (int k = wave; k < nk; k += W)
+      conv_load4_lds(row0 + lane < n ? a.nbr + (size_t)(k0 + k) * a.nbr_ld + row0 + lane : minus1 + lane,
+                     __builtin_amdgcn_readfirstlane(base + k * 256));
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (W > 1) __syncthreads();
+    uint32_t todo = 0;   // offsets at which some row has a neighbour
+#pragma unroll 9
+    for (int k = 0; k < nk; ++k) todo |= (__ballot(idx[k * 64 + lane] >= 0) != 0 ? 1u : 0u) << k;
+    todo = __builtin_amdgcn_readfirstlane(todo);
+    // this wave's share: every W-th stage
+    const int all = (__popc(todo) + S::OFFS - 1) / S::OFFS, stages = (all - wave + W - 1) / W;
+    auto drop = [&](int n_offsets) {
+      for (int i = 0; i < n_offsets; ++i) todo &= todo - 1;
+    };
+    drop(wave * S::OFFS);
+
+    // issues the loads of the next stage in `todo` into ring slot `slot`
+    auto issue = [&](int slot) {
+      const uint32_t buf = __builtin_amdgcn_readfirstlane(base + ring + slot * S::BYTES);
+      const int ka = __ffs(todo) - 1;
+      todo &= todo - 1;
+      int kb = ka;
+      bool second = true;
+      if constexpr (S::OFFS == 2) {   // (a second offset may not exist: zeros)
+        second = todo != 0;
+        if (second) kb = __ffs(todo) - 1;
+        todo &= todo - 1;
+      }
+      drop((W - 1) * S::OFFS);
+#pragma unroll
+      for (int q = 0; q < S::GLOADS; ++q) {
+        const int i = q < S::CH ? idx[ka * 64 + grow[q % S::CH]] : idx[kb * 64 + grow[q % S::CH]];
+        const bool have = i >= 0 && (q < S::CH || second);
+        const char* src = have ? a.x + (size_t)(uint32_t)i * a.x_ld_bytes : a.zrow;
+        conv_load16_lds(src + gchunk[q % S::CH], buf + q * 1024);
+      }
+      const char* wa = reinterpret_cast<const char*>(a.wfrag) + (size_t)(k0 + ka) * (BPR * 512) * mtiles;
+      const uint8_t* sa = wscales + (size_t)(k0 + ka) * (BPR * 32) * mtiles;
+      const uint32_t dk = (uint32_t)(kb - ka) * (BPR * 32) * mtiles;   // scale bytes from the first offset's units to the second's
+#pragma unroll
+      for (int q = 0; q < S::WLOADS; ++q)
+        conv_load16_lds(wa, wunit[q] * 512 + ln * 16 + (S::OFFS == 2 && 2 * q + lh >= MT ? dk * 16 : 0u), buf + S::WOFF + q * 1024);
+#pragma unroll
+      for (int q = 0; q < S::SLOADS; ++q)
+        conv_load4_lds(sa, sunit[q] * 32 + (lane & 7) * 4 + (S::OFFS == 2 && 8 * q + lane / 8 >= MT ? dk : 0u), buf + S::SOFF + q * 256);
+    };
+    if (stages > 0) issue(0);
+    int slot = 0;
+    for (int j = 0; j < stages; ++j) {
+      // the slot refilled here was read in the round before; its reads have returned
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (j + 1 < stages) {
+        issue(slot ^ 1);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::LOADS) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      const char* sb = lds + ring + slot * S::BYTES;
+#pragma unroll
+      for (int s = 0; s < S::KS; ++s) {
+        const int blk = 2 * s + lh;
+        const bool in = S::SB % 2 == 0 || blk < S::SB;
+        const int b = in ? blk : 0;
+        uint4 x[2];
+        uint32_t xs[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int r = 32 * u + ln;
+          const int cc = BPR == 1 ? 0 : b, sc = BPR;   // chunks of the codes and of the scales
+          const int cp = S::CH == 2 ? cc ^ ((r >> 3) & 1) : S::CH == 4 ? cc ^ ((r >> 2) & 3) : cc;
+          const int sp = S::CH == 2 ? sc ^ ((r >> 3) & 1) : S::CH == 4 ? sc ^ ((r >> 2) & 3) : sc;
+          const char* row = sb + (BPR == 1 ? b * S::CH * 1024 : 0) + r * S::CH * 16;
+          x[u] = *reinterpret_cast<const uint4*>(row + cp * 16);
+          xs[u] = *reinterpret_cast<const uint8_t*>(row + sp * 16 + (BPR == 1 ? 0 : b));
+          if (!in) xs[u] = 0;
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          const uint4 w = *reinterpret_cast<const uint4*>(sb + S::WOFF + ((b * MT + t) * 32 + ln) * 16);
+          uint32_t ws = *reinterpret_cast<const uint8_t*>(sb + S::SOFF + (b * MT + t) * 32 + ln);
+          if (!in) ws = 0;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) acc[t][u] = conv_mma(w, ws, x[u], xs[u], acc[t][u]);
+        }
+      }
+      slot ^= 1;
+    }
+  }
+  // Store through LDS, 32 rows at a time: a lane of the accumulators holds 4 channels of a row, a store takes 8 of one row
+  // and adds the waves' sums.  (Every load has been waited for; the rings are free.)
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  float* mine = reinterpret_cast<float*>(lds + ring);
+  constexpr int LPR = 4 * MT, RPP = 64 * W / LPR;   // threads per row, rows per pass
+  const int part = threadIdx.x % LPR, co = 32 * t0 + part * 8;
+  const bool wide = co < ((a.cout + 15) & ~15);
+  float4 b4[2], sc4;
+  if (wide) {
+    epilogue_consts<1>(a, co, &b4[0], &sc4);
+    epilogue_consts<1>(a, co + 4, &b4[1], &sc4);
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    if (W > 1 && u) __syncthreads();
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<v4f*>(mine + ln * S::PAD + t * 32 + q * 8 + lh * 4) =
+            v4f{acc[t][u][4 * q], acc[t][u][4 * q + 1], acc[t][u][4 * q + 2], acc[t][u][4 * q + 3]};
+    if (W > 1) __syncthreads();
+    for (int r = threadIdx.x / LPR; r < 32; r += RPP) {
+      const uint32_t row = row0 + 32 * u + r;
+      if (row >= n || !wide) continue;
+      float y[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float* src = reinterpret_cast<const float*>(lds + S::RING) + r * S::PAD + part * 8 + 4 * h;
+        v4f sum = *reinterpret_cast<const v4f*>(src);
+#pragma unroll
+        for (int w = 1; w < W; ++w) {
+          const v4f other = *reinterpret_cast<const v4f*>(src + w * (S::WAVE / 4));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sum[j] += other[j];
+        }
+        float v[4];
+        epilogue_values<1, MODE>(a, row, co + 4 * h, sum, b4[h], sc4, a.res ? residual_ptr(a, row, co + 4 * h) : nullptr, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[4 * h + j] = v[j];
+      }
+      if (MODE == 0 && a.out_dtype == SCN_DTYPE_INT8) {
+        const char4 q[2] = {pack_int8(a, y), pack_int8(a, y + 4)};
+        __builtin_memcpy(a.out + (size_t)row * a.out_ld + co, q, 8);
+      } else {
+        const v4h q[2] = {pack_fp16(y), pack_fp16(y + 4)};
+        __builtin_memcpy(reinterpret_cast<_Float16*>(a.out) + (size_t)row * a.out_ld + co, q, 16);
+      }
+    }
+  }
+}
+
+template <int BPR, int MT, int W, int MODE>
+static void launch_gather(ConvArgs& a, const uint8_t* ws, int mtiles, hipStream_t stream) {
+  const unsigned tiles = (a.n_bound + 63u) / 64u;
+  hipLaunchKernelGGL((k_conv_mx_gather<BPR, MT, W, MODE>), dim3(((tiles + 7u) / 8u) * 8u, (unsigned)(mtiles + MT - 1) / MT),
+                     dim3(64 * W), 0, stream, a, ws, mtiles);
+}
+
+// Waves per 64 rows.  One wave per tile has the fewest instructions and fills the GPU when there are many tiles; few tiles are
+// bound by the latency of a wave's chain of stages, which more waves shorten.  us with 1 / 2 / 4 waves: 120,000 rows 64 -> 64
+// 23.5 / 28.4 / 28.1, 20,000 rows 17.5 / 12.7 / 9.5, 12,254 rows 32 -> 64 13.3 / 9.0 / 7.4; with 128 output channels 48,460 rows
+// 64 -> 128 23.6 / 17.7 / 20.9, 120,000 rows 47.1 / 33.8 / 43.0, 60,000 rows 128 -> 128 35.0 / 38.2 / 46.4.
+// The choice follows the bound of the row count, never the count or what an earlier forward had: the order of the sums, and
+// so their last bit, depends on it.
+template <int BPR, int MODE>
+static void launch_gather(ConvArgs& a, const uint8_t* ws, int mtiles, hipStream_t stream) {
+  const int waves = a.n_bound <= 32768 ? 4 : a.n_bound <= 65536 ? 2 : 1;
+  if (mtiles > 2) launch_gather<BPR, 4, 2, MODE>(a, ws, mtiles, stream);
+  else if (mtiles == 2 && waves == 4) launch_gather<BPR, 2, 4, MODE>(a, ws, mtiles, stream);
+  else if (mtiles == 2 && waves == 2) launch_gather<BPR, 2, 2, MODE>(a, ws, mtiles, stream);
+  else if (mtiles == 2) launch_gather<BPR, 2, 1, MODE>(a, ws, mtiles, stream);
+  else if (waves == 4) launch_gather<BPR, 1, 4, MODE>(a, ws, mtiles, stream);
+  else if (waves == 2) launch_gather<BPR, 1, 2, MODE>(a, ws, mtiles, stream);
+  else launch_gather<BPR, 1, 1, MODE>(a, ws, mtiles, stream);
+}
+
+template <int BPR>
+static bool dispatch_gather(ConvArgs& a, const uint8_t* ws, int mtiles, hipStream_t stream) {
+  const bool half = !a.acc && a.out_dtype == SCN_DTYPE_FP16;
+  if (half && !a.res) launch_gather<BPR, 2>(a, ws, mtiles, stream);
+  else if (half && a.res_dtype == SCN_DTYPE_FP16 && a.mid_dtype == SCN_DTYPE_FP16 && a.a_rq_r == 0.f && a.b_rq_r == 0.f)
+    launch_gather<BPR, 4>(a, ws, mtiles, stream);
+  else launch_gather<BPR, 0>(a, ws, mtiles, stream);
+  return true;
+}
+
 bool conv_dispatch_mx(const ConvWeights& w, uint32_t n_hint, ConvArgs& a, hipStream_t stream) {
   (void)n_hint;
   a.wfrag = w.wfrag.as<uint4>();
   const uint8_t* ws = w.wscale.as<uint8_t>();
   const int mtiles = (w.cout + 31) / 32;
+  switch (w.chunks) {
+    case 1: return dispatch_gather<1>(a, ws, mtiles, stream);
+    case 2: return dispatch_gather<2>(a, ws, mtiles, stream);
+    case 3: return dispatch_gather<3>(a, ws, mtiles, stream);
+    case 4: return dispatch_gather<4>(a, ws, mtiles, stream);
+    default: break;
+  }
   const unsigned tiles = (a.n_bound + 127u) / 128u, blocks = ((tiles + 7u) / 8u) * 8u;
   const int mt = mtiles >= 4 ? 4 : mtiles;
   const dim3 grid(blocks, (unsigned)((mtiles + mt - 1) / mt));

@@ -127,11 +127,11 @@ struct ConvWeights {
   int mtiles = 0;   // ceil(cout / 16)
   int steps = 0;    // MFMA K-steps = ceil(kvol * chunks / 4)
   uint32_t cin_pad = 0;  // padded input channels the kernel expects (elements); MXFP4: bytes of an input row
-  DevBuf wfrag;     // [steps][mtiles][64] x 16 bytes, MFMA A-operand order (MXFP4: 32x32 tiles, ceil(cout / 32) of them)
+  DevBuf wfrag;     // [steps][mtiles][64] x 16 bytes, MFMA A-operand order (MXFP4: see init_mx)
   int mtiles32 = 0, steps32 = 0;
   DevBuf zrow;      // 512 bytes of zeros, then 64 words of -1
   DevBuf wfrag32;   // cout > 16: [steps32][mtiles32][64] x 16 bytes, A-operand order of the 32x32 MFMA
-  DevBuf wscale;    // fp32 [cout_pad]: s_w[c] (int8) or 1; MXFP4: scale bytes [steps][tiles][64]
+  DevBuf wscale;    // fp32 [cout_pad]: s_w[c] (int8) or 1; MXFP4: scale bytes
   DevBuf bias;      // fp32 [cout_pad]
   bool init(const uint16_t* w_fp16, const int shape[5], const float* ranges, const uint16_t* bias_fp16, int prec);
   bool init_mx(const uint16_t* w_fp16, const uint16_t* bias_fp16);   // MXFP4 packing, after set_geometry

@@ -371,6 +371,33 @@ def test_convolution(cin, cout, n, ks, stride, pad, subm):
     R.within(got, want, tol)
 
 
+@pytest.mark.parametrize("bound", [40000, 70000])
+@pytest.mark.parametrize("cin, cout, n, ks, stride, pad, subm", [CONVS[i] for i in (0, 2, 3, 4, 6, 7, 8, 10, 15)])
+def test_convolution_with_a_large_bound(cin, cout, n, ks, stride, pad, subm, bound):
+    """The bound of the row count chooses how many waves share a tile of rows; the count stays on the device."""
+    mx = _mx()
+    rng = np.random.default_rng(cin * 7 + cout + n)
+    grid = (9, 24, 21)
+    coords = scene(rng, n, grid)
+    out_coords, table = R.neighbours(coords, grid, ks, stride, pad, (1, 1, 1), subm)
+    idx = torch.zeros((bound, 4), dtype=torch.int32, device=DEV)
+    idx[:n, 1:] = torch.from_numpy(coords.astype(np.int32)).to(DEV)
+    num = torch.tensor([n], dtype=torch.int32, device=DEV)
+    kv, n_out = int(np.prod(ks)), table.shape[1]
+    rb = mx.Rulebook(bound, bound, kv)
+    rb.build_subm(idx, grid, ks, num=num) if subm else rb.build_sparse(idx, grid, ks, stride, pad, num=num)
+    w = (rng.standard_normal((cout, *ks, cin)) / np.sqrt(4 * cin)).astype(np.float16)
+    b = rng.standard_normal(cout).astype(np.float16)
+    x = rows(rng, n, cin)
+    q = mx.MxRows.empty(bound, cin, DEV)
+    mx.quantize_rows(torch.cat([torch.from_numpy(x), torch.full((bound - n, cin), float("nan"), dtype=torch.float16)]).to(DEV), num=num, out=q)
+    y, mag = R.convolution(R.fake(x), R.fake(w.reshape(cout * kv, cin)).reshape(cout, kv, cin), b.astype(np.float64), table)
+    out = torch.full((bound, -(-cout // 16) * 16), 3.0, dtype=torch.float16, device=DEV)
+    mx.Conv(w, b).forward(q, rb, bound, out=out)
+    R.within(out[:n_out, :cout].double().cpu().numpy(), y, R.tolerance(y, mag, kv * cin, 2.0 ** -11))
+    assert (out[n_out:] == 3).all()
+
+
 def test_convolution_nan_rows_reach_their_neighbours_only():
     mx = _mx()
     rng = np.random.default_rng(3)
