@@ -206,6 +206,26 @@ def test_product(m, n, k, x):
         R.within(got.double().cpu().numpy(), y, R.tolerance(y, mag, k, HALF[out_dtype]))
 
 
+# enough tiles of 128 x 128, then of 256 x 256, for the GPU; k of one stage, of a short last stage, of a short scale span
+@pytest.mark.parametrize("m, n, k", [(2050, 2061, 96), (2177, 2049, 515), (5000, 1030, 256), (4100, 4111, 290), (4097, 4300, 777), (16400, 1290, 1024),
+                                     (4111, 4099, 2080)])
+def test_large_products(m, n, k):
+    mx = _mx()
+    rng = np.random.default_rng(m + n + k)
+    w, wv = mx_rows(rng, n, k)
+    a, av = mx_rows(rng, m, k)
+    res = rng.standard_normal((m, n)).astype(np.float16)
+    bias = rng.standard_normal(n).astype(np.float32)
+    y, mag = R.product(av, wv, bias, False, res, True)
+    for out_dtype in (torch.float16, torch.float32):
+        out = strided(np.full((m, n), 9, NP[out_dtype]), n + 3, 1)
+        num = torch.tensor([m - 130], dtype=torch.int32, device=DEV)
+        mx.product(a, w, bias=torch.from_numpy(bias).to(DEV), residual=torch.from_numpy(res).to(DEV), relu_after_add=True, out=out, num=num)
+        got = out.double().cpu().numpy()
+        R.within(got[:m - 130], y[:m - 130], R.tolerance(y, mag, k, HALF[out_dtype])[:m - 130])
+        assert (got[m - 130:] == 9).all()
+
+
 @pytest.mark.parametrize("m", [5, 60, 400])
 def test_product_device_count_strides_and_untouched_memory(m):
     mx = _mx()
