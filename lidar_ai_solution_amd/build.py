@@ -29,7 +29,7 @@ def sources():
 # Kernels whose memory waits are counted by hand (s_waitcnt vmcnt(N) names which load has landed): a register spill
 # adds scratch loads to that counter behind the code's back, so a build in which one of them uses scratch memory fails.
 # The compiler reports every kernel's resources as remarks; they are read from the output of these translation units.
-NO_SCRATCH_KERNELS = ("k_conv_lds",)   # (k_conv_tile and k_conv_rows leave their waits to the compiler)
+NO_SCRATCH_KERNELS = ("k_conv_lds", "k_conv_mx_gather", "k_mx_product_lds")   # (k_conv_tile and k_conv_rows leave their waits to the compiler)
 RESOURCE_REMARKS = "-Rpass-analysis=kernel-resource-usage"
 
 
@@ -104,7 +104,7 @@ def build(verbose: bool = False, jobs: int = 0, incremental: bool = False) -> st
     for src in sources():
         obj = os.path.join(obj_dir, os.path.basename(src) + ".o")
         objs.append(obj)
-        remarks = [RESOURCE_REMARKS] if os.path.basename(src).startswith("scn_conv_") else []
+        remarks = [RESOURCE_REMARKS] if os.path.basename(src).startswith(("scn_conv_", "scn_mx")) else []
         cmd = ["hipcc", *compile_flags, *remarks, "-I" + os.path.join(ROOT, "include"), "-c", src, "-o", obj]
         if incremental and not _stale(obj, src, cmd):
             continue

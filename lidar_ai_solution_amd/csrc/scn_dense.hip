@@ -55,6 +55,7 @@ int convert_rows(const void* in, int in_dtype, uint32_t in_c, uint32_t in_ld, fl
     return mx_quantize_rows(in, in_dtype, in_c, in_ld, in_range, relu, codes, out_ld, codes + mx_blocks(in_c) * kMxBlockBytes,
                             out_ld, n, n_dev, stream);
   }
+  SCN_REQUIRE(in_dtype != SCN_DTYPE_MXFP4, SCN_ERR_INVALID, "convert_rows: microscaled rows are read by scn_mx_dequantize_rows");
   const float in_scale = in_range > 0.f ? in_range / 127.f : 1.f;
   const float out_scale = out_range > 0.f ? 127.f / out_range : 1.f;
   if (n == 0) return SCN_OK;

@@ -102,3 +102,5 @@ def test_conversion_to_microscaled_rows_refuses_short_rows():
     L = capi.lib()
     assert L.scn_convert_rows(GOOD, capi.DTYPE_FP16, 64, 64, 0.0, GOOD, capi.DTYPE_MXFP4, 0, 47, 0.0, 0, 5, None, None) == 1
     assert b"needs 48 bytes" in L.scn_last_error()
+    assert L.scn_convert_rows(GOOD, capi.DTYPE_MXFP4, 64, 48, 0.0, GOOD, capi.DTYPE_FP16, 64, 64, 0.0, 0, 5, None, None) == 1
+    assert b"scn_mx_dequantize_rows" in L.scn_last_error()
