@@ -144,8 +144,15 @@ int conv_forward(const ConvWeights& w, const int32_t* nbr, uint32_t nbr_ld, cons
               w.cin_pad);
   SCN_REQUIRE(((size_t)io.x_ld * esz) % 16 == 0 && ((uintptr_t)io.x_dev & 15) == 0, SCN_ERR_INVALID,
               "conv: input rows must be 16-byte aligned");
-  SCN_REQUIRE(io.out_dtype == SCN_DTYPE_INT8 || io.out_dtype == SCN_DTYPE_FP16, SCN_ERR_INVALID, "conv: bad out dtype");
-  SCN_REQUIRE(io.out_ld >= (uint32_t)w.mtiles * 16, SCN_ERR_INVALID, "conv: output row stride %u < %d", io.out_ld,
+  const bool mx_only = io.out_dtype == SCN_DTYPE_MXFP4;   // microscaled rows instead of fp16 ones
+  SCN_REQUIRE(io.out_dtype == SCN_DTYPE_INT8 || io.out_dtype == SCN_DTYPE_FP16 || mx_only, SCN_ERR_INVALID, "conv: bad out dtype");
+  const uint32_t mx_bytes = mx_row_bytes((uint32_t)w.cout);
+  if (mx_only) {
+    SCN_REQUIRE(conv_stores_mx(w), SCN_ERR_UNSUPPORTED, "conv: microscaled output needs an mxfp4 layer of at most 128 input channels");
+    SCN_REQUIRE(io.out_ld >= mx_bytes && io.out_ld % 16 == 0 && ((uintptr_t)io.out_dev & 15) == 0, SCN_ERR_INVALID,
+                "conv: microscaled output rows of %d channels need %u bytes, 16-byte aligned (stride %u)", w.cout, mx_bytes, io.out_ld);
+  }
+  SCN_REQUIRE(mx_only || io.out_ld >= (uint32_t)w.mtiles * 16, SCN_ERR_INVALID, "conv: output row stride %u < %d", io.out_ld,
               w.mtiles * 16);
   const int osz = io.out_dtype == SCN_DTYPE_INT8 ? 1 : 2;
   SCN_REQUIRE(((size_t)io.out_ld * osz) % (4 * osz) == 0 && ((uintptr_t)io.out_dev & 7) == 0, SCN_ERR_INVALID,
@@ -182,9 +189,18 @@ int conv_forward(const ConvWeights& w, const int32_t* nbr, uint32_t nbr_ld, cons
   auto r_of = [](float range) { return range > 0.f ? 127.f / range : 0.f; };
   a.x_scale = s_of(io.x_dynamic_range);
   a.relu = io.relu;
-  a.out_dtype = io.out_dtype;
+  a.out_dtype = mx_only ? SCN_DTYPE_FP16 : io.out_dtype;
   a.out_r = r_of(io.out_dynamic_range);
-  a.out = (char*)io.out_dev;
+  a.out = mx_only ? nullptr : (char*)io.out_dev;
+  if (mx_only) {
+    a.mx_out = (char*)io.out_dev;
+    a.mx_ld = io.out_ld;
+  } else if (plan && plan->mx_out && conv_stores_mx(w) && io.out_dtype == SCN_DTYPE_FP16) {
+    SCN_REQUIRE(plan->mx_ld >= mx_bytes && plan->mx_ld % 16 == 0 && ((uintptr_t)plan->mx_out & 15) == 0, SCN_ERR_INVALID,
+                "conv: microscaled output rows misaligned or too short");
+    a.mx_out = (char*)plan->mx_out;
+    a.mx_ld = plan->mx_ld;
+  }
   a.out_ld = io.out_ld;
   a.acc = io.acc_dev;
   a.res = (const char*)io.res_dev;

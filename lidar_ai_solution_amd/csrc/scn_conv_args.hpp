@@ -50,6 +50,10 @@ struct ConvArgs {
   const uint32_t* perm = nullptr;
   const uint4* wfrag32 = nullptr;  // weights in 32x32 MFMA fragment order, steps32 K-steps
   int steps32 = 0;
+  // microscaled output (MXFP4 layers of up to 128 input channels): rows in the one-buffer form, of the values as the fp16
+  // output holds them; `out` may then be null
+  char* mx_out = nullptr;
+  uint32_t mx_ld = 0;
 };
 
 // What a convolution launch may use of a rulebook's tile plan.
@@ -57,6 +61,9 @@ struct PlanView {
   const uint32_t* tmask = nullptr;
   const uint32_t* perm = nullptr;   // nullptr: plan order = row order
   const int32_t* nbr = nullptr;     // table in plan order (sorted plans), else nullptr
+  // not of a plan: a second output of an MXFP4 layer, the microscaled rows of what it stores (see ConvArgs)
+  void* mx_out = nullptr;
+  uint32_t mx_ld = 0;
 };
 
 // Launch the kernel for these weights (one definition per element type, each in its own translation unit).
@@ -64,6 +71,8 @@ struct PlanView {
 bool conv_dispatch_int8(const ConvWeights& w, uint32_t n_hint, ConvArgs& a, hipStream_t stream);
 bool conv_dispatch_fp16(const ConvWeights& w, uint32_t n_hint, ConvArgs& a, hipStream_t stream);
 bool conv_dispatch_mx(const ConvWeights& w, uint32_t n_hint, ConvArgs& a, hipStream_t stream);
+// MXFP4 layers whose kernel can store microscaled rows.
+inline bool conv_stores_mx(const ConvWeights& w) { return w.precision == SCN_PRECISION_MXFP4 && w.chunks <= 4; }
 // Shapes the tile-plan kernel covers (narrow layers: input rows of at most 64 bytes, at most 64 output channels).
 bool conv_tile_covers(const ConvWeights& w);
 

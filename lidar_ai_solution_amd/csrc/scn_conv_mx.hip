@@ -1,6 +1,7 @@
 // Convolution on microscaled 4-bit rows (MXFP4): gathered rows x weights on the scaled matrix instructions.
 #include "scn_conv_kernels.hpp"
 #include "scn_mx.hpp"
+#include "scn_mx_device.hpp"
 
 namespace scn {
 
@@ -271,10 +272,11 @@ __global__ __launch_bounds__(64 * W, 2) void k_conv_mx_gather(const ConvArgs a, 
     if (W > 1) __syncthreads();
     for (int r = threadIdx.x / LPR; r < 32; r += RPP) {
       const uint32_t row = row0 + 32 * u + r;
-      if (row >= n || !wide) continue;
-      float y[8];
+      if (row >= n) continue;
+      float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        if (!wide) break;
         const float* src = reinterpret_cast<const float*>(lds + S::RING) + r * S::PAD + part * 8 + 4 * h;
         v4f sum = *reinterpret_cast<const v4f*>(src);
 #pragma unroll
@@ -290,10 +292,33 @@ __global__ __launch_bounds__(64 * W, 2) void k_conv_mx_gather(const ConvArgs a, 
       }
       if (MODE == 0 && a.out_dtype == SCN_DTYPE_INT8) {
         const char4 q[2] = {pack_int8(a, y), pack_int8(a, y + 4)};
-        __builtin_memcpy(a.out + (size_t)row * a.out_ld + co, q, 8);
-      } else {
-        const v4h q[2] = {pack_fp16(y), pack_fp16(y + 4)};
-        __builtin_memcpy(reinterpret_cast<_Float16*>(a.out) + (size_t)row * a.out_ld + co, q, 16);
+        if (wide) __builtin_memcpy(a.out + (size_t)row * a.out_ld + co, q, 8);
+        continue;
+      }
+      const v4h q[2] = {pack_fp16(y), pack_fp16(y + 4)};
+      if (wide && a.out) __builtin_memcpy(reinterpret_cast<_Float16*>(a.out) + (size_t)row * a.out_ld + co, q, 16);
+      if (a.mx_out) {   // microscaled rows of the fp16 values: 4 lanes hold a block
+        const int blocks = (a.cout + 31) / 32, b = co / 32;
+        float v[8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          v[j] = co + j < a.cout ? (float)q[j / 4][j % 4] : 0.f;
+          top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+        }
+        top = lanes_max<4>(top);
+        const uint32_t e = mx_scale_byte(top);
+        const float up = __uint_as_float((254u - (e == 255u ? 0u : e)) << 23);
+        if (b < blocks) {
+          char* dst = a.mx_out + (size_t)row * a.mx_ld;
+          *reinterpret_cast<uint32_t*>(dst + b * 16 + (part & 3) * 4) = e == 255u ? 0u : mx_codes8(v, up);
+          if ((part & 3) == 0) {
+            uint8_t* sc = reinterpret_cast<uint8_t*>(dst + blocks * 16);
+            sc[b] = (uint8_t)e;
+            if (b + 1 == blocks)
+              for (int z = blocks; z % 4 != 0; ++z) sc[z] = 0;
+          }
+        }
       }
     }
   }

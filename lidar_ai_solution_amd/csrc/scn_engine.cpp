@@ -151,6 +151,7 @@ struct Step {
   int relu2 = 0;
   bool conv_input_is_converted = false;
   int t_conv_in = -1;  // tensor or conversion buffer index actually read
+  int t_out_mx = -1;   // MXFP4 conv: conversion buffer that also receives the output, as microscaled rows
   // add
   float add_a_rq = 0.f, add_b_rq = 0.f;
   // dense
@@ -608,14 +609,38 @@ static bool build_engine(scn_engine& e) {
             st.label += "+relu";
           }
         }
+        // What MXFP4 convolutions read of an fp16 output, this one stores itself, as microscaled rows of the fp16 values
+        // (the same bits as the conversion step would give): beside the fp16 rows, or instead of them when nobody else
+        // reads those.
+        bool only_mx = false;
+        if (!keep_all && conv_stores_mx(*w) && out_dtype == SCN_DTYPE_FP16) {
+          size_t readers = 0;
+          for (auto& c : plan.consumers[t_out])
+            if (nodes[c.first].op == Op::Conv && plan.comp[c.first] == SCN_PRECISION_MXFP4 && nodes[c.first].wshape[4] == cout) ++readers;
+          if (readers > 0) {
+            only_mx = readers == plan.consumers[t_out].size() && !graph_outputs.count(t_out);
+            e.tensors.emplace_back();
+            RtTensor& cv = e.tensors.back();
+            cv.dtype = SCN_DTYPE_MXFP4;
+            cv.c = cout;
+            cv.ld = ((uint32_t)((cout + 31) / 32) * 16 + (((uint32_t)((cout + 31) / 32) + 3u) & ~3u) + 15u) & ~15u;
+            cv.coord = slot.coord_out;
+            cv.materialised = true;
+            st.t_out_mx = (int)e.tensors.size() - 1;
+            char keybuf[128];
+            snprintf(keybuf, sizeof(keybuf), "%d:%d:%a:%u", t_out, SCN_DTYPE_MXFP4, 0.0, cv.ld);
+            conversions[keybuf] = st.t_out_mx;
+          }
+        }
         RtTensor& o = e.tensors[t_out];
         o.dtype = out_dtype;
         o.range = out_range;
         o.c = cout;
         o.ld = (uint32_t)w->mtiles * 16;
         o.coord = slot.coord_out;
-        o.materialised = true;
-        st.t_out = t_out;
+        o.materialised = !only_mx;
+        st.t_out = only_mx ? st.t_out_mx : t_out;
+        if (only_mx) st.t_out_mx = -1;
         e.convs.push_back(std::move(w));
         e.steps.push_back(st);
         break;
@@ -906,10 +931,11 @@ static int allocate_runtime(scn_engine& e) {
     const Step& st = e.steps[si];
     for (int t : {st.t_in, st.t_in2, st.t_conv_in})
       if (t >= 0 && t < (int)e.tensors.size()) dies[t] = std::max(dies[t], (int)si);
-    if (st.t_out >= 0 && st.t_out < (int)e.tensors.size()) {
-      born[st.t_out] = std::min(born[st.t_out], (int)si);
-      dies[st.t_out] = std::max(dies[st.t_out], (int)si);
-    }
+    for (int t : {st.t_out, st.t_out_mx})
+      if (t >= 0 && t < (int)e.tensors.size()) {
+        born[t] = std::min(born[t], (int)si);
+        dies[t] = std::max(dies[t], (int)si);
+      }
   }
   for (int o : e.outputs) dies[o] = never;
   struct Shared {
@@ -1149,8 +1175,12 @@ static int run_step(scn_engine& e, Step& st, hipStream_t stream) {
           pv.nbr = tp.nbr.as<int32_t>();
         }
       }
+      if (st.t_out_mx >= 0) {
+        pv.mx_out = e.tensors[st.t_out_mx].data;
+        pv.mx_ld = e.tensors[st.t_out_mx].ld;
+      }
       return conv_forward(*e.convs[st.conv], s.rb.nbr.as<int32_t>(), s.rb.ld, s.rb.n_out_dev(), s.rb.n_bound_out,
-                          s.rb.n_out_hint(), io, stream, planned ? &pv : nullptr);
+                          s.rb.n_out_hint(), io, stream, planned || pv.mx_out ? &pv : nullptr);
     }
     case StepKind::Add: {
       const RtTensor& a = e.tensors[st.t_in];

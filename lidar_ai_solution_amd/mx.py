@@ -327,9 +327,11 @@ class Conv:
         self.cout, self.cin = int(w.shape[0]), int(w.shape[4])
 
     def forward(self, x: MxRows, rulebook: Rulebook, max_rows: int, relu: bool = False, residual: Optional[torch.Tensor] = None,
-                relu_after_add: bool = False, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+                relu_after_add: bool = False, out=None, stream=None):
         """x: MxRows in the one-buffer form (what quantize_rows makes).  Returns fp16 [max_rows, Cout]; rows beyond the
-        rulebook's count are left as they were.  residual: fp16 [max_rows, >= Cout rounded up to 16]."""
+        rulebook's count are left as they were.  residual: fp16 [max_rows, >= Cout rounded up to 16].  out: fp16 rows of at
+        least Cout rounded up to 16 channels, or MxRows in the one-buffer form, which get the rows that quantize_rows would
+        make of the fp16 result (layers of at most 128 input channels)."""
         blocks = (self.cin + 31) // 32
         if rulebook.rows_in is None:
             raise ValueError("the rulebook has not been built")
@@ -337,8 +339,10 @@ class Conv:
             raise ValueError(f"the rulebook covers {rulebook.rows_in} input rows and up to {rulebook.rows_out} output rows")
         if x.channels != self.cin:
             raise ValueError(f"input rows have {x.channels} channels, the weight expects {self.cin}")
-        if x.codes_ld != x.scales_ld or x.scales_ptr != x.codes_ptr + 16 * blocks:
-            raise ValueError("the convolution reads rows in the one-buffer form (codes, then scales)")
+        to_mx = isinstance(out, MxRows)
+        for r, b in ((x, blocks),) + (((out, (self.cout + 31) // 32),) if to_mx else ()):
+            if r.codes_ld != r.scales_ld or r.scales_ptr != r.codes_ptr + 16 * b:
+                raise ValueError("the convolution reads and writes rows in the one-buffer form (codes, then scales)")
         wide = (self.cout + 15) // 16 * 16
         if stream is not None:
             with _using(stream, x.index):
@@ -348,6 +352,10 @@ class Conv:
                 return self.forward(x, rulebook, max_rows, relu, residual, relu_after_add, out)
         if out is None:
             out, out_ld = torch.empty((max_rows, wide), dtype=torch.float16, device="cuda"), wide
+        elif to_mx:
+            out_ld = out.codes_ld
+            if out.num_rows < max_rows or out.channels != self.cout or out.index != x.index:
+                raise ValueError(f"out must hold {max_rows} rows of {self.cout} channels on cuda:{x.index}")
         else:
             out_ld = _check_rows(out, (torch.float16,), "out")
             if out.shape[0] < max_rows or out.shape[1] < wide:
@@ -355,7 +363,8 @@ class Conv:
             _same_device(x.index, out)
         io = capi.ConvIO()
         io.x_dev, io.x_ld = x.codes_ptr, x.codes_ld
-        io.relu, io.out_dtype, io.out_dev, io.out_ld = int(bool(relu)), capi.DTYPE_FP16, out.data_ptr(), out_ld
+        io.relu, io.out_ld = int(bool(relu)), out_ld
+        io.out_dtype, io.out_dev = (capi.DTYPE_MXFP4, out.codes_ptr) if to_mx else (capi.DTYPE_FP16, out.data_ptr())
         if residual is not None:
             io.res_ld = _check_rows(residual, (torch.float16,), "residual")
             if residual.shape[0] < max_rows or residual.shape[1] < wide:
@@ -364,7 +373,7 @@ class Conv:
             io.res_dev, io.res_dtype, io.mid_dtype = residual.data_ptr(), capi.DTYPE_FP16, capi.DTYPE_FP16
             io.relu_after_add = int(bool(relu_after_add))
         capi.check(_lib().scn_conv_forward(self._h, rulebook._h, C.byref(io), _stream(x.index)))
-        if out.shape == (max_rows, self.cout):
+        if to_mx or out.shape == (max_rows, self.cout):
             return out
         return out[:max_rows, :self.cout]
 

@@ -418,6 +418,25 @@ def test_convolution_with_a_large_bound(cin, cout, n, ks, stride, pad, subm, bou
     assert (out[n_out:] == 3).all()
 
 
+@pytest.mark.parametrize("cin, cout, n, ks, stride, pad, subm", [c for c in CONVS if c[0] <= 128])
+def test_convolution_stores_microscaled_rows(cin, cout, n, ks, stride, pad, subm):
+    """out = MxRows gets, bit for bit, what quantize_rows makes of the fp16 result (also of results that are not finite)."""
+    mx = _mx()
+    rng = np.random.default_rng(cin + cout * 5 + n)
+    rb, table, n_out, conv, _, _ = conv_case(rng, n, (9, 24, 21), cin, cout, ks, stride, pad, subm)
+    x = rows(rng, n, cin)
+    x[n // 2] = np.nan
+    q = mx.quantize_rows(torch.from_numpy(x).to(DEV))
+    res = torch.from_numpy(rng.standard_normal((n_out, -(-cout // 16) * 16)).astype(np.float16)).to(DEV)
+    for kw in (dict(relu=True), dict(residual=res, relu_after_add=True)):
+        want = mx.quantize_rows(conv.forward(q, rb, n_out, **kw))
+        got = mx.MxRows.empty(n_out + 3, cout, DEV)
+        got.codes.fill_(0xAA), got.scales.fill_(0xBB)
+        assert conv.forward(q, rb, n_out, out=got, **kw) is got
+        assert torch.equal(got.codes[:n_out], want.codes) and torch.equal(got.scales[:n_out], want.scales)
+        assert (got.codes[n_out:] == 0xAA).all() and (got.scales[n_out:] == 0xBB).all()
+
+
 def test_convolution_nan_rows_reach_their_neighbours_only():
     mx = _mx()
     rng = np.random.default_rng(3)
@@ -463,6 +482,11 @@ def test_convolution_refusals():
         conv.forward(mx.quantize_rows(torch.zeros((49, 64), dtype=torch.float16, device=DEV)), rb, n_out)
     with pytest.raises(ValueError):
         conv.forward(q, mx.Rulebook(50, 50, 27), n_out)
+    wide = mx.Conv(np.zeros((32, 3, 3, 3, 160), np.float16))
+    with pytest.raises(RuntimeError):                                     # microscaled output of a wide layer
+        wide.forward(mx.quantize_rows(torch.zeros((50, 160), dtype=torch.float16, device=DEV)), rb, n_out, out=mx.MxRows.empty(n_out, 32, DEV))
+    with pytest.raises(ValueError):
+        conv.forward(q, rb, n_out, out=mx.MxRows.empty(n_out, 64, DEV))
     with pytest.raises(RuntimeError):                                     # kernel volume
         mx.Conv(np.zeros((32, 1, 1, 1, 64), np.float16)).forward(q, rb, n_out)
 
