@@ -97,11 +97,11 @@ bool ConvWeights::init(const uint16_t* w_fp16, const int shape[5], const float* 
 }
 
 // Weights of a convolution on microscaled rows: block g (kernel offset, block of the row) of the 32 output channels of a
-// tile is one unit of 32 x 16 code bytes, wfrag[g][tile][channel]; their scale bytes wscale[g][tile][channel].
+// tile is one unit of 32 x 16 code bytes, wfrag[g][tile][channel]; the scale bytes of 4 tiles one word, wscale[g][tile / 4][channel][tile % 4].
 bool ConvWeights::init_mx(const uint16_t* w_fp16, const uint16_t* bias_fp16) {
   const int tiles = (cout + 31) / 32;
-  const size_t units = (size_t)kvol * chunks * tiles;
-  std::vector<uint8_t> frag(units * 32 * 16, 0), sc(units * 32, 0);
+  const size_t blocks = (size_t)kvol * chunks, groups = (tiles + 3) / 4;
+  std::vector<uint8_t> frag(blocks * tiles * 32 * 16, 0), sc(blocks * groups * 32 * 4, 0);
   std::vector<float> bs((size_t)tiles * 32, 0.f);
   if (bias_fp16)
     for (int c = 0; c < cout; ++c) bs[c] = half_bits_to_float(bias_fp16[c]);
@@ -111,7 +111,7 @@ bool ConvWeights::init_mx(const uint16_t* w_fp16, const uint16_t* bias_fp16) {
       const int k = g / chunks, b = g % chunks, nv = std::min(32, cin - 32 * b);
       for (int i = 0; i < nv; ++i) v[i] = half_bits_to_float(w_fp16[((size_t)co * kvol + k) * cin + 32 * b + i]);
       const size_t f = ((size_t)g * tiles + co / 32) * 32 + co % 32;
-      sc[f] = mx_quantize_block(v, nv, &frag[f * 16]);
+      sc[(((size_t)g * groups + co / 128) * 32 + co % 32) * 4 + co / 32 % 4] = mx_quantize_block(v, nv, &frag[f * 16]);
     }
   if (!zrow.alloc(1536) || !wfrag.alloc(frag.size()) || !wscale.alloc(sc.size()) || !bias.alloc(bs.size() * 4)) return false;
   if (hipMemset(zrow.p, 0, 512) != hipSuccess || hipMemset(zrow.as<char>() + 512, 0xFF, 1024) != hipSuccess ||

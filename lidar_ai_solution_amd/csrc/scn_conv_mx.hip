@@ -10,10 +10,12 @@ typedef int v8i __attribute__((ext_vector_type(8)));
 // v_mfma_scale_f32_32x32x64_f8f6f4 with 4-bit operands: lane l supplies row / column l % 32, the 16 code bytes of K-block
 // l / 32 and that block's scale.  Rows of A are output channels, columns of B voxels (as in the other convolution kernels); a
 // K-step takes two blocks.  Weights are laid out in units of one block x 32 output channels: wfrag[block][tile][32] x 16
-// bytes, scale bytes wscales[block][tile][32]; block g = kernel offset * BPR + block of the row (BPR = blocks of an input row).
+// bytes; the scale bytes of 4 tiles are one word, wscales[block][tile / 4][32][4]; block g = kernel offset * BPR + block of the
+// row (BPR = blocks of an input row).  SEL: the byte of ws.
+template <int SEL>
 __device__ __forceinline__ v16f conv_mma(const uint4& w, uint32_t ws, const uint4& x, uint32_t xs, v16f c) {
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v8i{(int)w.x, (int)w.y, (int)w.z, (int)w.w, 0, 0, 0, 0},
-                                                         v8i{(int)x.x, (int)x.y, (int)x.z, (int)x.w, 0, 0, 0, 0}, c, 4, 4, 0,
+                                                         v8i{(int)x.x, (int)x.y, (int)x.z, (int)x.w, 0, 0, 0, 0}, c, 4, 4, SEL,
                                                          (int)ws, 0, (int)xs);
 }
 
@@ -50,8 +52,10 @@ __global__ __launch_bounds__(256) void k_conv_mx_rows(const ConvArgs a, const ui
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      const size_t f = ((size_t)min(g, total - 1) * mtiles + min(t0 + t, mtiles - 1)) * 32 + ln;
-      acc[t] = conv_mma(a.wfrag[f], wscales[f], xq, xs, acc[t]);
+      const size_t g0 = (size_t)min(g, total - 1);
+      const int tt = min(t0 + t, mtiles - 1);
+      acc[t] = conv_mma<0>(a.wfrag[(g0 * mtiles + tt) * 32 + ln], wscales[((g0 * ((mtiles + 3) / 4) + tt / 4) * 32 + ln) * 4 + tt % 4],
+                           xq, xs, acc[t]);
     }
   }
   if (row >= n) return;
@@ -73,9 +77,8 @@ __global__ __launch_bounds__(256) void k_conv_mx_rows(const ConvArgs a, const ui
 // A workgroup owns 64 rows and MT tiles of 32 output channels; its W waves share the rows' neighbour indices and deal the
 // kernel offsets out between them, so a wave only ever waits for its own loads; the waves' sums are added (in wave order) when
 // the rows are stored.
-//   a stage = one kernel offset that some row has a neighbour at (two of them for rows of one block): 64 gathered rows and
-//   the weights of its blocks; a wave fetches one stage ahead (two ahead leave room for fewer waves: 120,000 rows 64 -> 64
-//   36.6 against 23.8 us).  Rows without a neighbour fetch zeros (scale 2^-127, codes 0).
+//   a stage = one kernel offset that some row has a neighbour at (two of them for rows of one block): 64 gathered rows in LDS and
+//   the weights of its blocks in registers (in LDS they leave room for fewer waves); a wave fetches one stage ahead.  Rows without a neighbour fetch zeros (scale 2^-127, codes 0).
 //   LDS rows of 3 and 5 chunks are read without bank conflicts as they are; rows of 2 and 4 chunks hold chunk c at position
 //   c ^ (row / 8) % 2 and c ^ (row / 4) % 4.
 template <int BPR, int MT, int W>
@@ -83,31 +86,18 @@ struct ConvMxStage {
   static constexpr int OFFS = BPR == 1 ? 2 : 1;                  // kernel offsets of a stage
   static constexpr int SB = BPR * OFFS, KS = (SB + 1) / 2;       // blocks and K-steps
   static constexpr int CH = BPR + 1;                             // 16-byte chunks of a row
-  static constexpr int GLOADS = CH * OFFS;                       // wave loads: 64 rows
-  static constexpr int WLOADS = (SB * MT + 1) / 2, SLOADS = (SB * MT + 7) / 8;   // weight units of 512 bytes, their scales
-  static constexpr int LOADS = GLOADS + WLOADS + SLOADS;
-  static constexpr int WOFF = GLOADS * 1024, SOFF = WOFF + WLOADS * 1024, BYTES = SOFF + SLOADS * 256;
-  static constexpr int KMAX = 27;                                // kernel offsets whose indices are held at a time
+  static constexpr int GLOADS = CH * OFFS, BYTES = GLOADS * 1024;   // wave loads: 64 rows
+  static constexpr int KMAX = 28;                                // kernel offsets whose indices are held at a time
   static constexpr int RING = KMAX * 256;                        // LDS offset of the rings
   static constexpr int PAD = 32 * MT + 4;                        // floats per row of the store buffer
   static constexpr int WAVE = 2 * BYTES > 32 * PAD * 4 ? 2 * BYTES : 32 * PAD * 4;
   static constexpr int LDS = RING + W * WAVE;
 };
 
-// 64 x 16 (or 64 x 4) bytes to LDS, lane l's to base + 16 l (4 l): in assembly, because the compiler would order its own LDS
+// 64 x 16 bytes to LDS, lane l's to base + 16 l: in assembly, because the compiler would order its own LDS
 // reads behind every such load in flight.  m0 has no other user in this kernel.
 __device__ __forceinline__ void conv_load16_lds(const void* src, uint32_t base) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(base) : "memory");
-}
-// (a wave's base and a 32-bit offset per lane)
-__device__ __forceinline__ void conv_load16_lds(const void* src, uint32_t offset, uint32_t base) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(src), "s"(base) : "memory");
-}
-__device__ __forceinline__ void conv_load4_lds(const void* src, uint32_t offset, uint32_t base) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(src), "s"(base) : "memory");
-}
-__device__ __forceinline__ void conv_load4_lds(const void* src, uint32_t base) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(base) : "memory");
 }
 
 // MODE: the epilogue (see epilogue_values): 2 and 4 are fp16 output without and with an fp16 residual, 0 everything.
@@ -134,8 +124,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_conv_mx_gather(const ConvArgs a, 
 #pragma unroll
       for (int j = 0; j < 16; ++j) acc[t][u][j] = 0.f;
 
-  // what this lane fetches of a stage: for gather load q (of one offset) the row and the chunk, for the weight and scale loads
-  // the unit (block and tile) counted from the offset's first block
+  // what this lane fetches of a stage: the row and the chunk of gather load q (of one offset); its weights are those of K-block
+  // 2 s + lh of step s
   int grow[S::CH], gchunk[S::CH];
 #pragma unroll
   for (int q = 0; q < S::CH; ++q) {
@@ -143,16 +133,18 @@ __global__ __launch_bounds__(64 * W, 2) void k_conv_mx_gather(const ConvArgs a, 
     grow[q] = r;
     gchunk[q] = (S::CH == 2 ? p ^ ((r >> 3) & 1) : S::CH == 4 ? p ^ ((r >> 2) & 3) : p) * 16;
   }
-  auto unit_of = [&](int u) {
-    u = min(u, S::SB * MT - 1);
-    const int b = u / MT, t = u - b * MT;
-    return (uint32_t)((BPR == 1 ? 0 : b) * mtiles + min(t0 + t, mtiles - 1));
-  };
-  uint32_t wunit[S::WLOADS], sunit[S::SLOADS];
+  // weights of one kernel offset: uint4 and scale words; this lane's of step s start at woff, soff (a block that does not exist
+  // takes another one's codes, and scales of 0)
+  const uint32_t wstride = BPR * mtiles * 32, sstride = BPR * ((mtiles + 3) / 4) * 32;
+  uint32_t woff[S::KS], soff[S::KS];
 #pragma unroll
-  for (int q = 0; q < S::WLOADS; ++q) wunit[q] = unit_of(2 * q + lh);
-#pragma unroll
-  for (int q = 0; q < S::SLOADS; ++q) sunit[q] = unit_of(8 * q + lane / 8);
+  for (int s = 0; s < S::KS; ++s) {
+    const int b = BPR == 1 || (S::SB % 2 && 2 * s + lh >= S::SB) ? 0 : 2 * s + lh;
+    woff[s] = (b * mtiles + t0) * 32 + ln;
+    soff[s] = (b * ((mtiles + 3) / 4) + t0 / 4) * 32 + ln;
+  }
+  uint4 w[S::KS][MT], w1[S::KS][MT];
+  uint32_t ws[S::KS], ws1[S::KS];
 
   for (int k0 = 0; k0 < a.kvol; k0 += S::KMAX) {
     // neighbour rows of up to KMAX offsets; rows beyond the count have none
@@ -160,14 +152,24 @@ __global__ __launch_bounds__(64 * W, 2) void k_conv_mx_gather(const ConvArgs a, 
     const int32_t* minus1 = reinterpret_cast<const int32_t*>(a.zrow + 512);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (W > 1 && k0) __syncthreads();   // (the indices before these have been read)
-    for (int k = wave; k < nk; k += W)
-      conv_load4_lds(row0 + lane < n ? a.nbr + (size_t)(k0 + k) * a.nbr_ld + row0 + lane : minus1 + lane,
-                     __builtin_amdgcn_readfirstlane(base + k * 256));
+    // one load: 4 offsets x 64 rows, 4 rows per lane (the table holds -1 from the count up to the next multiple of 32 rows)
+    for (int k4 = wave * 4; k4 < nk; k4 += W * 4) {
+      const int k = k0 + k4 + (lane >> 4);
+      const uint32_t row = row0 + (lane & 15) * 4;
+      conv_load16_lds(k4 + (lane >> 4) < nk && row < n ? a.nbr + (size_t)k * a.nbr_ld + row : minus1 + lane * 4,
+                      __builtin_amdgcn_readfirstlane(base + k4 * 256));
+    }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (W > 1) __syncthreads();
     uint32_t todo = 0;   // offsets at which some row has a neighbour
-#pragma unroll 9
-    for (int k = 0; k < nk; ++k) todo |= (__ballot(idx[k * 64 + lane] >= 0) != 0 ? 1u : 0u) << k;
+#pragma unroll
+    for (int k4 = 0; k4 < S::KMAX; k4 += 4) {
+      if (k4 >= nk) break;
+      const int4 v = reinterpret_cast<const int4*>(idx)[k4 * 16 + lane];
+      const uint64_t some = __ballot((v.x & v.y & v.z & v.w) >= 0);   // (indices are -1 or not negative: the sign of their AND)
+      todo |= ((some & 0xFFFFull ? 1u : 0u) | (some & 0xFFFF0000ull ? 2u : 0u) | (some & 0xFFFF00000000ull ? 4u : 0u) |
+               (some >> 48 ? 8u : 0u)) << k4;
+    }
     todo = __builtin_amdgcn_readfirstlane(todo);
     // this wave's share: every W-th stage
     const int all = (__popc(todo) + S::OFFS - 1) / S::OFFS, stages = (all - wave + W - 1) / W;
@@ -176,7 +178,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_conv_mx_gather(const ConvArgs a, 
     };
     drop(wave * S::OFFS);
 
-    // issues the loads of the next stage in `todo` into ring slot `slot`
+    // issues the loads of the next stage in `todo`: rows into ring slot `slot`, weights into w1 and ws1
     auto issue = [&](int slot) {
       const uint32_t buf = __builtin_amdgcn_readfirstlane(base + ring + slot * S::BYTES);
       const int ka = __ffs(todo) - 1;
@@ -189,34 +191,42 @@ __global__ __launch_bounds__(64 * W, 2) void k_conv_mx_gather(const ConvArgs a, 
         todo &= todo - 1;
       }
       drop((W - 1) * S::OFFS);
+      int i[S::GLOADS];
+#pragma unroll
+      for (int q = 0; q < S::GLOADS; ++q) i[q] = idx[(q < S::CH ? ka : kb) * 64 + grow[q % S::CH]];
+      // (uniform bases, 32-bit offsets per lane)
+      const char* wp = reinterpret_cast<const char*>(a.wfrag) + (size_t)(k0 + ka) * wstride * 16;
+      const char* sp = reinterpret_cast<const char*>(wscales) + (size_t)(k0 + ka) * sstride * 4;
+      const uint32_t other = S::OFFS == 2 && lh ? (uint32_t)(kb - ka) : 0u;
+#pragma unroll
+      for (int s = 0; s < S::KS; ++s) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+          w1[s][t] = *reinterpret_cast<const uint4*>(wp + (woff[s] + other * wstride + min(t, mtiles - 1 - t0) * 32) * 16);
+        ws1[s] = *reinterpret_cast<const uint32_t*>(sp + (soff[s] + other * sstride) * 4);
+      }
 #pragma unroll
       for (int q = 0; q < S::GLOADS; ++q) {
-        const int i = q < S::CH ? idx[ka * 64 + grow[q % S::CH]] : idx[kb * 64 + grow[q % S::CH]];
-        const bool have = i >= 0 && (q < S::CH || second);
-        const char* src = have ? a.x + (size_t)(uint32_t)i * a.x_ld_bytes : a.zrow;
-        conv_load16_lds(src + gchunk[q % S::CH], buf + q * 1024);
+        const char* row = a.x + (size_t)(uint32_t)max(i[q], 0) * a.x_ld_bytes;
+        row = i[q] >= 0 && (q < S::CH || second) ? row : a.zrow;
+        conv_load16_lds(row + gchunk[q % S::CH], buf + q * 1024);
       }
-      const char* wa = reinterpret_cast<const char*>(a.wfrag) + (size_t)(k0 + ka) * (BPR * 512) * mtiles;
-      const uint8_t* sa = wscales + (size_t)(k0 + ka) * (BPR * 32) * mtiles;
-      const uint32_t dk = (uint32_t)(kb - ka) * (BPR * 32) * mtiles;   // scale bytes from the first offset's units to the second's
-#pragma unroll
-      for (int q = 0; q < S::WLOADS; ++q)
-        conv_load16_lds(wa, wunit[q] * 512 + ln * 16 + (S::OFFS == 2 && 2 * q + lh >= MT ? dk * 16 : 0u), buf + S::WOFF + q * 1024);
-#pragma unroll
-      for (int q = 0; q < S::SLOADS; ++q)
-        conv_load4_lds(sa, sunit[q] * 32 + (lane & 7) * 4 + (S::OFFS == 2 && 8 * q + lane / 8 >= MT ? dk : 0u), buf + S::SOFF + q * 256);
     };
     if (stages > 0) issue(0);
     int slot = 0;
     for (int j = 0; j < stages; ++j) {
-      // the slot refilled here was read in the round before; its reads have returned
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (j + 1 < stages) {
-        issue(slot ^ 1);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::LOADS) : "memory");
-      } else {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      // everything of this stage has landed, and the reads of the slot that is refilled now have returned (the wait is one the
+      // compiler knows, so that it adds none for the weights)
+      __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0)
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int s = 0; s < S::KS; ++s) {
+        ws[s] = ws1[s];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) w[s][t] = w1[s][t];
       }
+      if (j + 1 < stages) issue(slot ^ 1);
+      __builtin_amdgcn_sched_barrier(0);
       const char* sb = lds + ring + slot * S::BYTES;
 #pragma unroll
       for (int s = 0; s < S::KS; ++s) {
@@ -236,13 +246,15 @@ __global__ __launch_bounds__(64 * W, 2) void k_conv_mx_gather(const ConvArgs a, 
           xs[u] = *reinterpret_cast<const uint8_t*>(row + sp * 16 + (BPR == 1 ? 0 : b));
           if (!in) xs[u] = 0;
         }
+        const uint32_t wsv = in ? ws[s] : 0u;
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          const uint4 w = *reinterpret_cast<const uint4*>(sb + S::WOFF + ((b * MT + t) * 32 + ln) * 16);
-          uint32_t ws = *reinterpret_cast<const uint8_t*>(sb + S::SOFF + (b * MT + t) * 32 + ln);
-          if (!in) ws = 0;
-#pragma unroll
-          for (int u = 0; u < 2; ++u) acc[t][u] = conv_mma(w, ws, x[u], xs[u], acc[t][u]);
+        for (int u = 0; u < 2; ++u) {
+          acc[0][u] = conv_mma<0>(w[s][0], wsv, x[u], xs[u], acc[0][u]);
+          if constexpr (MT > 1) acc[1][u] = conv_mma<1>(w[s][1], wsv, x[u], xs[u], acc[1][u]);
+          if constexpr (MT > 2) {
+            acc[2][u] = conv_mma<2>(w[s][2], wsv, x[u], xs[u], acc[2][u]);
+            acc[3][u] = conv_mma<3>(w[s][3], wsv, x[u], xs[u], acc[3][u]);
+          }
         }
       }
       slot ^= 1;
@@ -331,16 +343,18 @@ static void launch_gather(ConvArgs& a, const uint8_t* ws, int mtiles, hipStream_
                      dim3(64 * W), 0, stream, a, ws, mtiles);
 }
 
-// Waves per 64 rows.  One wave per tile has the fewest instructions and fills the GPU when there are many tiles; few tiles are
-// bound by the latency of a wave's chain of stages, which more waves shorten.  us with 1 / 2 / 4 waves: 120,000 rows 64 -> 64
-// 23.5 / 28.4 / 28.1, 20,000 rows 17.5 / 12.7 / 9.5, 12,254 rows 32 -> 64 13.3 / 9.0 / 7.4; with 128 output channels 48,460 rows
-// 64 -> 128 23.6 / 17.7 / 20.9, 120,000 rows 47.1 / 33.8 / 43.0, 60,000 rows 128 -> 128 35.0 / 38.2 / 46.4.
+// Waves per 64 rows.  Few tiles are bound by the latency of a wave's chain of stages, which more waves shorten; where the tiles
+// of one wave just fill the GPU (12 per CU), one has the fewest instructions; beyond that two balance better.  us with 1 / 2 / 4
+// waves: 20,000 rows 64 -> 64 14.1 / 10.9 / 8.2, 120,000 rows 22.9 / 26.6 / 25.9, 260,000 rows 45.7 / 41.1 / 45.4; with 128
+// output channels (twice the work per wave) 20,000 rows 128 -> 128 26.3 / 20.1 / 15.9, 48,460 rows 64 -> 128 20.8 / 17.2 / 19.1,
+// 150,000 rows 128 -> 128 68.1 / 60.0 / 63.0.
 // The choice follows the bound of the row count, never the count or what an earlier forward had: the order of the sums, and
 // so their last bit, depends on it.
 template <int BPR, int MODE>
 static void launch_gather(ConvArgs& a, const uint8_t* ws, int mtiles, hipStream_t stream) {
-  const int waves = a.n_bound <= 32768 ? 4 : a.n_bound <= 65536 ? 2 : 1;
-  if (mtiles > 2) launch_gather<BPR, 4, 2, MODE>(a, ws, mtiles, stream);
+  const int waves = a.n_bound <= 32768 ? 4 : a.n_bound <= 65536 || a.n_bound > 196608 || mtiles > 2 ? 2 : 1;
+  if (mtiles > 2 && waves == 4) launch_gather<BPR, 4, 4, MODE>(a, ws, mtiles, stream);
+  else if (mtiles > 2) launch_gather<BPR, 4, 2, MODE>(a, ws, mtiles, stream);
   else if (mtiles == 2 && waves == 4) launch_gather<BPR, 2, 4, MODE>(a, ws, mtiles, stream);
   else if (mtiles == 2 && waves == 2) launch_gather<BPR, 2, 2, MODE>(a, ws, mtiles, stream);
   else if (mtiles == 2) launch_gather<BPR, 2, 1, MODE>(a, ws, mtiles, stream);

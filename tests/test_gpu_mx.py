@@ -391,7 +391,7 @@ def test_convolution(cin, cout, n, ks, stride, pad, subm):
     R.within(got, want, tol)
 
 
-@pytest.mark.parametrize("bound", [40000, 70000])
+@pytest.mark.parametrize("bound", [40000, 70000, 200000])
 @pytest.mark.parametrize("cin, cout, n, ks, stride, pad, subm", [CONVS[i] for i in (0, 2, 3, 4, 6, 7, 8, 10, 15)])
 def test_convolution_with_a_large_bound(cin, cout, n, ks, stride, pad, subm, bound):
     """The bound of the row count chooses how many waves share a tile of rows; the count stays on the device."""
