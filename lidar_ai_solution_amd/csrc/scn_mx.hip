@@ -514,28 +514,39 @@ __device__ __forceinline__ v16f mx_mma32_sel(const v4i& a, uint32_t sa, const v4
                                                          c, 4, 4, SEL, (int)sa, SEL, (int)sb);
 }
 
-template <int BN, int BM, int TN, int TM>
+// KS > 1: as many groups of waves share a tile, each with a run of the stages and LDS of its own, and add their sums when the
+// tile is stored: a few tiles down a long k are bound by the latency of a stage (0.37 us), of which KS then pass at a time
+// (100 x 100 x 8192: 14.1 us with one group, 11.3 us with 2, 10.5 us with 4).  The order of the sums is fixed.
+template <int BN, int BM, int TN, int TM, int KS>
 struct ProductTile {
   static constexpr int WN = BN / (32 * TN), WM = BM / (32 * TM), WAVES = WN * WM;
   static constexpr int STAGE = (BN + BM) * 128, SPAN = (BN + BM) * 16;   // bytes of LDS per stage of codes, per span of scales
   static constexpr int PAD = 32 * TN + 4;                             // floats per row of the store buffer
   static constexpr int STORE = WAVES * 32 * PAD * 4;
-  static size_t lds(uint32_t stages) { return std::max<size_t>((stages > 1 ? 2 : 1) * (size_t)STAGE + (stages > 2 ? 2 : 1) * SPAN, STORE); }
+  static_assert(KS == 1 || (TN == 1 && TM == 1), "split sums are added tile by tile");
+  // bytes of LDS of a group that runs through `stages` stages
+  __host__ __device__ static uint32_t lds(uint32_t stages) {
+    const uint32_t need = (stages > 1 ? 2 : 1) * STAGE + (stages > 2 ? 2 : 1) * SPAN;
+    return need > (uint32_t)STORE ? need : (uint32_t)STORE;
+  }
+  // stages of a group (whole spans of scales) when all have `stages`
+  __host__ __device__ static uint32_t share(uint32_t stages) { return KS == 1 ? stages : ((stages + KS - 1) / KS + 1) / 2 * 2; }
 };
 
-template <int BN, int BM, int TN, int TM>
-constexpr int kProductThreads = 64 * ProductTile<BN, BM, TN, TM>::WAVES;
+template <int BN, int BM, int TN, int TM, int KS>
+constexpr int kProductThreads = 64 * ProductTile<BN, BM, TN, TM, KS>::WAVES * KS;
 
-template <int BN, int BM, int TN, int TM>
-__global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_product_lds(const ProductArgs p, uint32_t tiles_n,
+template <int BN, int BM, int TN, int TM, int KS>
+__global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM, KS>), 2) void k_mx_product_lds(const ProductArgs p, uint32_t tiles_n,
                                                                                               uint32_t tiles_m) {
-  using T = ProductTile<BN, BM, TN, TM>;
+  using T = ProductTile<BN, BM, TN, TM, KS>;
   constexpr int WAVES = T::WAVES, STAGE = T::STAGE, SPAN = T::SPAN;
   constexpr int LOADS = (BN + BM) / 8 / WAVES;   // wave loads per stage of codes
   static_assert(LOADS * 8 * WAVES == BN + BM && BN % (WAVES * 8) == 0 && WAVES % 2 == 0 && BN % 64 == 0 && BN + BM <= WAVES * 64,
                 "a wave's load is all weights or all rows, and one load per wave fetches a span of scales");
   extern __shared__ __align__(16) char lds[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = wave_all % WAVES, group = wave_all / WAVES;
   const int ln = lane & 31, lh = lane >> 5;
   const uint32_t m = eff_n(p.m_dev, p.m);
   // XCD x takes the x-th contiguous eighth of the tiles (each XCD has its own L2), in bands of 8 row tiles that are walked
@@ -552,8 +563,11 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
   // What this lane fetches: code load q covers 8 rows (lane / 8), position lane % 8; the scale load 64 rows.  A wave's load is
   // all weights or all rows, so an address is a wave's base, which advances from stage to stage, and a lane's offset.
   uint32_t coff[LOADS];
-  const uint8_t* wcode = p.b + (size_t)n0 * p.b_ld;
-  const uint8_t* xcode = (const uint8_t*)p.a + (size_t)i0 * p.a_ld;
+  // this group's run of blocks: kb of them from `first` on (none, for the last groups, when there are few)
+  const uint32_t all = (p.kb + 7) / 8, share = T::share(all), first = min(group * share * 8, p.kb);
+  const uint32_t kb = min(p.kb - first, share * 8);
+  const uint8_t* wcode = p.b + (size_t)n0 * p.b_ld + (size_t)first * 16;
+  const uint8_t* xcode = (const uint8_t*)p.a + (size_t)i0 * p.a_ld + (size_t)first * 16;
   const uint32_t last_w = p.n - 1 - n0, last_x = m - 1 - i0;   // rows of this tile that exist
   const uint32_t cblk = (lane & 7) ^ ((wave * 4 + (lane >> 4)) & 7);   // block of a stage this lane fetches
 #pragma unroll
@@ -563,17 +577,19 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
   }
   const uint32_t srow = (wave * 64) % (BN + BM);               // (the small tile has fewer rows than lanes: some are loaded twice)
   const bool s_is_w = srow < BN;
-  const uint8_t* sbase = s_is_w ? p.bs + (size_t)n0 * p.bs_ld : p.as + (size_t)i0 * p.as_ld;
+  const uint8_t* sbase = (s_is_w ? p.bs + (size_t)n0 * p.bs_ld : p.as + (size_t)i0 * p.as_ld) + first;
   const uint32_t s_ld = s_is_w ? p.bs_ld : p.as_ld, srow0 = s_is_w ? srow : srow - BN, last_s = s_is_w ? last_w : last_x;
   const uint32_t soff = min(srow0 + lane, last_s) * s_ld;
-  const uint32_t stages = (p.kb + 7) / 8, words = (p.kb + 3) / 4;   // stages of 8 blocks, scale words of 4; the last may be shorter
-  const uint32_t base = (uint32_t)(uintptr_t)(mx_lptr)lds;
-  const uint32_t span0 = (stages > 1 ? 2 : 1) * STAGE;              // LDS offset of the scales
+  const uint32_t stages = (kb + 7) / 8, words = (kb + 3) / 4;   // stages of 8 blocks, scale words of 4; the last may be shorter
+  const uint32_t most = min(share, all);                        // stages of the first group
+  char* const lds_g = lds + (KS > 1 ? group * T::lds(most) : 0);
+  const uint32_t base = (uint32_t)(uintptr_t)(mx_lptr)lds_g;
+  const uint32_t span0 = (most > 1 ? 2 : 1) * STAGE;            // LDS offset of the scales
   // Loads [from, to) of a wave's LOADS of stage st.  In a stage of fewer than 8 blocks a lane whose block does not exist
   // fetches the first one instead: the masked scales (2^-127 on both sides) take it out of the sums.
   auto load = [&](uint32_t st, int from, int to) {
     const uint32_t buf = __builtin_amdgcn_readfirstlane(base + (st & 1) * STAGE);
-    const uint32_t back = st * 8 + cblk < p.kb ? 0u : cblk * 16;
+    const uint32_t back = st * 8 + cblk < kb ? 0u : cblk * 16;
 #pragma unroll
     for (int q = 0; q < LOADS; ++q)
       if (q >= from && q < to)
@@ -608,7 +624,7 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
   uint2 ws[TN], xs[TM], ws1[TN], xs1[TM];
   // operands of step S (64 channels) of stage st
   auto read = [&](uint32_t st, int S, v4i(&wv)[TN], v4i(&xv)[TM]) {
-    const char* sb = lds + (st & 1) * STAGE;
+    const char* sb = lds_g + (st & 1) * STAGE;
     const uint32_t pos = ((2 * S + lh) ^ swz) * 16;
 #pragma unroll
     for (int a = 0; a < TN; ++a) wv[a] = *reinterpret_cast<const v4i*>(sb + (w_row + 32 * a) * 128 + pos);
@@ -617,7 +633,7 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
   };
   // the scale words of a stage; take_scales: blocks 2 s + lh of step s are bytes 0 and 2 of the words after a shift by lh bytes
   auto read_scales = [&](uint32_t st) {
-    const char* sb = lds + span0 + ((st >> 1) & 1) * SPAN + (st & 1) * 8;
+    const char* sb = lds_g + span0 + ((st >> 1) & 1) * SPAN + (st & 1) * 8;
 #pragma unroll
     for (int a = 0; a < TN; ++a) ws1[a] = *reinterpret_cast<const uint2*>(sb + (w_row + 32 * a) * 16);
 #pragma unroll
@@ -643,9 +659,11 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
   for (int a = 0; a < TN; ++a) w[1][a] = v4i{0, 0, 0, 0}, ws[a] = make_uint2(0, 0);
 #pragma unroll
   for (int b = 0; b < TM; ++b) x[1][b] = v4i{0, 0, 0, 0}, xs[b] = make_uint2(0, 0);
-  load_scales(0);
-  load(0, 0, LOADS);
   uint32_t st = 0;
+  if (KS == 1 || stages > 0) {
+    load_scales(0);
+    load(0, 0, LOADS);
+  }
 #pragma unroll 1
   for (; st + 1 < stages; ++st) {
     SCN_MX_BARRIER()
@@ -686,9 +704,9 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
       if (want && row < m) __builtin_memcpy(&pre[q], (const _Float16*)p.res + (size_t)row * p.res_ld + ch, 16);
     }
   }
-  {   // the last stage, of 1 .. 8 blocks
+  if (KS == 1 || stages > 0) {   // the last stage, of 1 .. 8 blocks
     SCN_MX_BARRIER()
-    const uint32_t left = p.kb - st * 8;
+    const uint32_t left = kb - st * 8;
     read_scales(st);
     take_scales(left >= 4 ? ~0u : (1u << (8 * left)) - 1u, left >= 8 ? ~0u : left > 4 ? (1u << (8 * (left - 4))) - 1u : 0u);
     read(st, 0, w[0], x[0]);
@@ -708,11 +726,13 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
   }
 #undef SCN_MX_MULTIPLY
 #undef SCN_MX_BARRIER
+  if constexpr (KS > 1)
+    for (uint32_t i = stages; i < most; ++i) __builtin_amdgcn_s_barrier();   // (one per stage of the first group)
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   // Store through LDS (wave-private, 32 rows at a time): a lane of the accumulators holds 4 consecutive channels of one
   // row, a store wants whole 128-byte lines of a row.
-  float* buf = reinterpret_cast<float*>(lds) + wave * 32 * T::PAD;
+  float* buf = reinterpret_cast<float*>(KS > 1 ? lds_g : lds) + wave * 32 * T::PAD;
 #pragma unroll
   for (int b = 0; b < TM; ++b) {
 #pragma unroll
@@ -721,25 +741,37 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM>), 2) void k_mx_pro
       for (int q = 0; q < 4; ++q)
         *reinterpret_cast<v4f*>(buf + ln * T::PAD + a * 32 + q * 8 + lh * 4) =
             v4f{acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]};
+    if constexpr (KS > 1) __syncthreads();
 #pragma unroll
     for (int r = 0; r < PASSES; ++r) {
       const uint32_t row = row0 + (b * PASSES + r) * RPP;
-      if (row < m && ch < p.n)
-        product_store8<PRE>(p, row, ch, buf + (r * RPP + lane / LPR) * T::PAD + (lane % LPR) * 8, pre[PRE ? b * PASSES + r : 0]);
+      if (row >= m || ch >= p.n || r % KS != group) continue;
+      float* src = buf + (r * RPP + lane / LPR) * T::PAD + (lane % LPR) * 8;
+      if constexpr (KS > 1) {   // the groups' sums, in their order; each pass is one group's to store
+        v4f y[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+        for (int g = 0; g < KS; ++g) {
+          const float* part = src + ((int)g - group) * (int)(T::lds(most) / 4);
+          y[0] += *reinterpret_cast<const v4f*>(part);
+          y[1] += *reinterpret_cast<const v4f*>(part + 4);
+        }
+        reinterpret_cast<v4f*>(src)[0] = y[0];
+        reinterpret_cast<v4f*>(src)[1] = y[1];
+      }
+      product_store8<PRE>(p, row, ch, src, pre[PRE ? b * PASSES + r : 0]);
     }
   }
 }
 
-template <int BN, int BM, int TN, int TM>
+template <int BN, int BM, int TN, int TM, int KS>
 static int launch_product(const ProductArgs& p, hipStream_t stream) {
-  using T = ProductTile<BN, BM, TN, TM>;
+  using T = ProductTile<BN, BM, TN, TM, KS>;
   const uint64_t tn = ((uint64_t)p.n + BN - 1) / BN, tm = ((uint64_t)p.m + BM - 1) / BM;
   SCN_REQUIRE((uint64_t)std::max(std::max(p.a_ld, p.b_ld), std::max(p.as_ld, p.bs_ld)) * 256 < (1ull << 32), SCN_ERR_UNSUPPORTED,
               "mx_product: rows more than 16 MB apart");
   SCN_REQUIRE(tn * tm < (1ull << 27), SCN_ERR_UNSUPPORTED, "mx_product: %u x %u outputs are too many for one call", p.m, p.n);
-  const size_t lds = T::lds((p.kb + 7) / 8);
-  hipLaunchKernelGGL((k_mx_product_lds<BN, BM, TN, TM>), dim3((unsigned)((tn * tm + 7) / 8 * 8)), dim3(64 * T::WAVES), lds, stream, p,
-                     (uint32_t)tn, (uint32_t)tm);
+  const uint32_t stages = (p.kb + 7) / 8;
+  hipLaunchKernelGGL((k_mx_product_lds<BN, BM, TN, TM, KS>), dim3((unsigned)((tn * tm + 7) / 8 * 8)), dim3(64 * T::WAVES * KS),
+                     KS * T::lds(std::min(T::share(stages), stages)), stream, p, (uint32_t)tn, (uint32_t)tm);
   return SCN_OK;
 }
 
@@ -830,11 +862,17 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
   // against 4.0 us, 4096 x 16384 24.5 against 36.6; but 8192 x 8192 24.6 against 20.3, 256 x 128 4.1 against 3.1
   else if (io.m <= 32 && kb >= 32 && io.n <= 4096) launch_few<SCN_DTYPE_MXFP4, 2>(p, stream);
   else {
-    // the largest tile of which there are enough for the GPU's 256 CUs
-    const uint64_t t256 = (uint64_t)ceil_div(io.n, 256) * ceil_div(io.m, 256), t128 = (uint64_t)ceil_div(io.n, 128) * ceil_div(io.m, 128);
-    int rc = t256 >= 256 && kb > 8 ? launch_product<256, 256, 4, 2>(p, stream)
-             : t128 >= 256         ? launch_product<128, 128, 2, 2>(p, stream)
-                                   : launch_product<64, 64, 1, 1>(p, stream);
+    // The largest tile of which there are enough for the GPU's 256 CUs, when k is long enough for its reuse to count.  us for
+    // 64 | 128 | 256 rows and channels a tile:
+    //   4096 x 3584 x 2048 38 | 27 | 22, 3584 x 3584 x 512 13.0 | 13.4 | 11.6, 2560 x 2560 x 2048 (100 tiles of 256) 19 | 14 | 18;
+    //   32640 x 128 x 2048 14.5 | 12.2 | 18.7, 32640 x 128 x 512 5.6 | 6.1 | 10.3, 100000 x 64 x 1024 15.5 | 20.8 | 28.8.
+    // The smallest tile with k in 4 parts, when there is a CU for every tile and 16 stages: whole | in 4 parts
+    //   4096 x 64 x 8192 13.6 | 10.4, 16384 x 64 x 4096 (256 tiles) 12.8 | 10.0; x 2048 6.4 | 6.5; 24576 x 64 x 4096 14 | 17.
+    const auto tiles = [&](uint32_t t) { return (uint64_t)ceil_div(io.n, t) * ceil_div(io.m, t); };
+    int rc = tiles(256) >= 144 && io.n > 128 && kb > 8   ? launch_product<256, 256, 4, 2, 1>(p, stream)
+             : tiles(128) >= 256 && io.n > 64 && kb > 16 ? launch_product<128, 128, 2, 2, 1>(p, stream)
+             : tiles(64) <= 256 && kb > 120              ? launch_product<64, 64, 1, 1, 4>(p, stream)
+                                                         : launch_product<64, 64, 1, 1, 1>(p, stream);
     if (rc) return rc;
   }
   SCN_HIP(hipGetLastError());

@@ -226,6 +226,30 @@ def test_large_products(m, n, k):
         assert (got[m - 130:] == 9).all()
 
 
+# tiles of 128 x 128 with many stages; few tiles down a long k, whose stages are divided: a short last part, an empty one
+# (17 stages), equal ones, a last stage of one block
+@pytest.mark.parametrize("m, n, k", [(2100, 2200, 1500), (65, 61, 3873), (64, 1000, 4100), (130, 300, 8192), (33, 70, 12289), (1000, 1, 4097)])
+@pytest.mark.parametrize("res_dtype", [np.float16, np.float32])
+def test_products_down_a_long_k(m, n, k, res_dtype):
+    mx = _mx()
+    rng = np.random.default_rng(m + n + k)
+    w, wv = mx_rows(rng, n, k)
+    a, av = mx_rows(rng, m, k)
+    res = rng.standard_normal((m, n)).astype(res_dtype)
+    bias = rng.standard_normal(n).astype(np.float32)
+    y, mag = R.product(av, wv, bias, True, res, False)
+    for out_dtype, kept in ((torch.float16, m), (torch.float32, m // 2), (torch.float16, 0)):
+        out = strided(np.full((m, n), 9, NP[out_dtype]), n + 3, 1)
+        num = torch.tensor([kept], dtype=torch.int32, device=DEV)
+        mx.product(a, w, bias=torch.from_numpy(bias).to(DEV), relu=True, residual=torch.from_numpy(res).to(DEV), out=out, num=num)
+        got = out.double().cpu().numpy()
+        R.within(got[:kept], y[:kept], R.tolerance(y, mag, k, HALF[out_dtype])[:kept])
+        assert (got[kept:] == 9).all()
+        again = torch.full_like(out, 9)
+        mx.product(a, w, bias=torch.from_numpy(bias).to(DEV), relu=True, residual=torch.from_numpy(res).to(DEV), out=again, num=num)
+        assert torch.equal(again, out)
+
+
 @pytest.mark.parametrize("m", [5, 60, 400])
 def test_product_device_count_strides_and_untouched_memory(m):
     mx = _mx()
