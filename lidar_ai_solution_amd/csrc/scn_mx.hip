@@ -421,8 +421,7 @@ __global__ __launch_bounds__(512) void k_mx_product_few(const ProductArgs p) {
 }
 
 // Bias, ReLU, residual and store of 8 consecutive channels of one row, from LDS (one 16-byte store in fp16, two in fp32;
-// rows of any alignment).  PRE: an fp16 residual has been loaded into `pre` already.
-template <bool PRE>
+// rows of any alignment).  `pre`: the fp16 residual, if there is one.
 __device__ __forceinline__ void product_store8(const ProductArgs& p, uint32_t i, uint32_t j, const float* src, const v4u pre) {
   if (j + 8 > p.n) {
 #pragma unroll 1
@@ -450,16 +449,14 @@ __device__ __forceinline__ void product_store8(const ProductArgs& p, uint32_t i,
     for (int q = 0; q < 8; ++q) y[q] = y[q] > 0.f ? y[q] : 0.f;
   }
   if (p.res) {
-    const size_t at = (size_t)i * p.res_ld + j;
     if (p.res_fp32) {
       float r[8];
-      __builtin_memcpy(r, (const float*)p.res + at, 32);
+      __builtin_memcpy(r, (const float*)p.res + (size_t)i * p.res_ld + j, 32);
 #pragma unroll
       for (int q = 0; q < 8; ++q) y[q] += r[q];
     } else {
       _Float16 r[8];
-      if constexpr (PRE) __builtin_memcpy(r, &pre, 16);
-      else __builtin_memcpy(r, (const _Float16*)p.res + at, 16);
+      __builtin_memcpy(r, &pre, 16);
 #pragma unroll
       for (int q = 0; q < 8; ++q) y[q] += (float)r[q];
     }
@@ -689,21 +686,24 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM, KS>), 2) void k_mx
     SCN_MX_MULTIPLY(0, 0, y)
   }
   SCN_MX_MULTIPLY(1, 2, y)
-  // what this lane will store, and the fp16 residual it needs there, fetched while the last stage travels (the kernel whose
-  // accumulators leave registers for it)
+  // What this lane will store, and the fp16 residual it needs there: fetched while the last stage travels where the
+  // accumulators leave registers for it, else 32 rows at a time in front of their stores.
   constexpr int LPR = 4 * TN, RPP = 64 / LPR, PASSES = 32 / RPP;   // lanes per row (8 channels each), rows per pass
-  constexpr bool PRE = TN * TM <= 4;
+  constexpr bool EARLY = TN * TM <= 4;
   const uint32_t row0 = i0 + wm * 32 * TM + lane / LPR, ch = n0 + wn * 32 * TN + (lane % LPR) * 8;
-  v4u pre[PRE ? TM * PASSES : 1];
-  if constexpr (PRE) {
+  v4u pre[EARLY ? TM * PASSES : PASSES];
+  auto residual = [&](int b, int to) {
     const bool want = p.res && !p.res_fp32 && ch + 8 <= p.n;
 #pragma unroll
-    for (int q = 0; q < TM * PASSES; ++q) {
-      pre[q] = v4u{0, 0, 0, 0};
-      const uint32_t row = row0 + q * RPP;
-      if (want && row < m) __builtin_memcpy(&pre[q], (const _Float16*)p.res + (size_t)row * p.res_ld + ch, 16);
+    for (int r = 0; r < PASSES; ++r) {
+      pre[to + r] = v4u{0, 0, 0, 0};
+      const uint32_t row = row0 + (b * PASSES + r) * RPP;
+      if (want && row < m) __builtin_memcpy(&pre[to + r], (const _Float16*)p.res + (size_t)row * p.res_ld + ch, 16);
     }
-  }
+  };
+  if constexpr (EARLY)
+#pragma unroll
+    for (int b = 0; b < TM; ++b) residual(b, b * PASSES);
   if (KS == 1 || stages > 0) {   // the last stage, of 1 .. 8 blocks
     SCN_MX_BARRIER()
     const uint32_t left = kb - st * 8;
@@ -735,6 +735,7 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM, KS>), 2) void k_mx
   float* buf = reinterpret_cast<float*>(KS > 1 ? lds_g : lds) + wave * 32 * T::PAD;
 #pragma unroll
   for (int b = 0; b < TM; ++b) {
+    if constexpr (!EARLY) residual(b, 0);
 #pragma unroll
     for (int a = 0; a < TN; ++a)
 #pragma unroll
@@ -757,7 +758,7 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM, KS>), 2) void k_mx
         reinterpret_cast<v4f*>(src)[0] = y[0];
         reinterpret_cast<v4f*>(src)[1] = y[1];
       }
-      product_store8<PRE>(p, row, ch, src, pre[PRE ? b * PASSES + r : 0]);
+      product_store8(p, row, ch, src, pre[(EARLY ? b * PASSES : 0) + r]);
     }
   }
 }
@@ -866,13 +867,16 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
     // 64 | 128 | 256 rows and channels a tile:
     //   4096 x 3584 x 2048 38 | 27 | 22, 3584 x 3584 x 512 13.0 | 13.4 | 11.6, 2560 x 2560 x 2048 (100 tiles of 256) 19 | 14 | 18;
     //   32640 x 128 x 2048 14.5 | 12.2 | 18.7, 32640 x 128 x 512 5.6 | 6.1 | 10.3, 100000 x 64 x 1024 15.5 | 20.8 | 28.8.
+    // With a residual whose size is beyond the caches' (16 M numbers) the wider stores of the larger tile count as well:
+    //   123646 x 256 x 128 31 | 28 | 31, 50000 x 256 x 128 10.6 | 13.2 | 12.7.
     // The smallest tile with k in 4 parts, when there is a CU for every tile and 16 stages: whole | in 4 parts
     //   4096 x 64 x 8192 13.6 | 10.4, 16384 x 64 x 4096 (256 tiles) 12.8 | 10.0; x 2048 6.4 | 6.5; 24576 x 64 x 4096 14 | 17.
     const auto tiles = [&](uint32_t t) { return (uint64_t)ceil_div(io.n, t) * ceil_div(io.m, t); };
-    int rc = tiles(256) >= 144 && io.n > 128 && kb > 8   ? launch_product<256, 256, 4, 2, 1>(p, stream)
-             : tiles(128) >= 256 && io.n > 64 && kb > 16 ? launch_product<128, 128, 2, 2, 1>(p, stream)
-             : tiles(64) <= 256 && kb > 120              ? launch_product<64, 64, 1, 1, 4>(p, stream)
-                                                         : launch_product<64, 64, 1, 1, 1>(p, stream);
+    const bool wide = kb > 16 || (io.res_dev && (uint64_t)io.m * io.n >= (16u << 20));
+    int rc = tiles(256) >= 144 && io.n > 128 && kb > 8 ? launch_product<256, 256, 4, 2, 1>(p, stream)
+             : tiles(128) >= 256 && io.n > 64 && wide  ? launch_product<128, 128, 2, 2, 1>(p, stream)
+             : tiles(64) <= 256 && kb > 120            ? launch_product<64, 64, 1, 1, 4>(p, stream)
+                                                       : launch_product<64, 64, 1, 1, 1>(p, stream);
     if (rc) return rc;
   }
   SCN_HIP(hipGetLastError());

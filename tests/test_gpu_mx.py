@@ -206,9 +206,9 @@ def test_product(m, n, k, x):
         R.within(got.double().cpu().numpy(), y, R.tolerance(y, mag, k, HALF[out_dtype]))
 
 
-# enough tiles of 128 x 128, then of 256 x 256, for the GPU; k of one stage, of a short last stage, of a short scale span
+# enough tiles of 128 x 128 or 256 x 256 for the GPU, and tiles of 64 x 64; k of one stage, of a short last stage, of a short scale span
 @pytest.mark.parametrize("m, n, k", [(2050, 2061, 96), (2177, 2049, 515), (5000, 1030, 256), (4100, 4111, 290), (4097, 4300, 777), (16400, 1290, 1024),
-                                     (4111, 4099, 2080)])
+                                     (4111, 4099, 2080), (16500, 1030, 70)])
 def test_large_products(m, n, k):
     mx = _mx()
     rng = np.random.default_rng(m + n + k)
