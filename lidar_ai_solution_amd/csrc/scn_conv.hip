@@ -149,6 +149,7 @@ int conv_forward(const ConvWeights& w, const int32_t* nbr, uint32_t nbr_ld, cons
   const uint32_t mx_bytes = mx_row_bytes((uint32_t)w.cout);
   if (mx_only) {
     SCN_REQUIRE(conv_stores_mx(w), SCN_ERR_UNSUPPORTED, "conv: microscaled output needs an mxfp4 layer of at most 128 input channels");
+    SCN_REQUIRE(io.out_dev != io.x_dev, SCN_ERR_INVALID, "conv: the output rows must not be the input rows");
     SCN_REQUIRE(io.out_ld >= mx_bytes && io.out_ld % 16 == 0 && ((uintptr_t)io.out_dev & 15) == 0, SCN_ERR_INVALID,
                 "conv: microscaled output rows of %d channels need %u bytes, 16-byte aligned (stride %u)", w.cout, mx_bytes, io.out_ld);
   }

@@ -769,9 +769,11 @@ static int launch_product(const ProductArgs& p, hipStream_t stream) {
   const uint64_t tn = ((uint64_t)p.n + BN - 1) / BN, tm = ((uint64_t)p.m + BM - 1) / BM;
   SCN_REQUIRE((uint64_t)std::max(std::max(p.a_ld, p.b_ld), std::max(p.as_ld, p.bs_ld)) * 256 < (1ull << 32), SCN_ERR_UNSUPPORTED,
               "mx_product: rows more than 16 MB apart");
-  SCN_REQUIRE(tn * tm < (1ull << 27), SCN_ERR_UNSUPPORTED, "mx_product: %u x %u outputs are too many for one call", p.m, p.n);
+  constexpr uint64_t threads = 64 * T::WAVES * KS;   // (a launch has fewer than 2^32 threads)
+  SCN_REQUIRE((tn * tm + 7) / 8 * 8 * threads < (1ull << 32), SCN_ERR_UNSUPPORTED, "mx_product: %u x %u outputs are too many for one call",
+              p.m, p.n);
   const uint32_t stages = (p.kb + 7) / 8;
-  hipLaunchKernelGGL((k_mx_product_lds<BN, BM, TN, TM, KS>), dim3((unsigned)((tn * tm + 7) / 8 * 8)), dim3(64 * T::WAVES * KS),
+  hipLaunchKernelGGL((k_mx_product_lds<BN, BM, TN, TM, KS>), dim3((unsigned)((tn * tm + 7) / 8 * 8)), dim3((unsigned)threads),
                      KS * T::lds(std::min(T::share(stages), stages)), stream, p, (uint32_t)tn, (uint32_t)tm);
   return SCN_OK;
 }
@@ -784,13 +786,15 @@ static size_t product_workspace(uint32_t m, uint32_t k) { return product_direct(
 
 // U = runs a wave requests at once: what it has to do in all, up to 8 (4 for two row tiles).
 template <int AT, int MT>
-static void launch_few(const ProductArgs& p, hipStream_t stream) {
+static int launch_few(const ProductArgs& p, hipStream_t stream) {
   const uint32_t runs = (p.kb + 3) / 4, waves = std::min(8u, runs), per = ceil_div(runs, waves);
+  SCN_REQUIRE(p.n < (1u << 27), SCN_ERR_UNSUPPORTED, "mx_product: %u x %u outputs are too many for one call", p.m, p.n);
   const dim3 grid(ceil_div(p.n, 16)), block(64 * waves);
   if (per == 1) hipLaunchKernelGGL((k_mx_product_few<AT, MT, 1>), grid, block, 0, stream, p);
   else if (per == 2) hipLaunchKernelGGL((k_mx_product_few<AT, MT, 2>), grid, block, 0, stream, p);
   else if (per <= 4 || MT > 1) hipLaunchKernelGGL((k_mx_product_few<AT, MT, 4>), grid, block, 0, stream, p);
   else hipLaunchKernelGGL((k_mx_product_few<AT, 1, 8>), grid, block, 0, stream, p);
+  return SCN_OK;
 }
 
 int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
@@ -809,9 +813,12 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
   auto aligned = [](const void* p, int dtype) { return ((uintptr_t)p & (dtype == SCN_DTYPE_FP32 ? 3 : 1)) == 0; };
   SCN_REQUIRE(io.out_dev && aligned(io.out_dev, io.out_dtype) && io.out_ld >= io.n, SCN_ERR_INVALID,
               "mx_product: null or misaligned output, or row stride %u < %u", io.out_ld, io.n);
+  SCN_REQUIRE(io.out_dev != io.a_dev, SCN_ERR_INVALID, "mx_product: the output must not be the rows");
   SCN_REQUIRE(aligned(io.bias_dev, io.bias_dtype), SCN_ERR_INVALID, "mx_product: misaligned bias");
   SCN_REQUIRE(!io.res_dev || (aligned(io.res_dev, io.res_dtype) && io.res_ld >= io.n), SCN_ERR_INVALID,
               "mx_product: misaligned residual, or row stride %u < %u", io.res_ld, io.n);
+  SCN_REQUIRE(io.res_dev != io.out_dev || (io.res_dtype == io.out_dtype && (io.res_ld == io.out_ld || io.m == 1)), SCN_ERR_INVALID,
+              "mx_product: an output that is the residual must have its type and row stride");
   ProductArgs p;
   p.a = io.a_dev;
   p.a_ld = io.a_ld;
@@ -856,12 +863,13 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
       at = SCN_DTYPE_MXFP4;
     }
   }
-  if (at == SCN_DTYPE_FP16) launch_few<SCN_DTYPE_FP16, 1>(p, stream);
-  else if (at == SCN_DTYPE_FP32) launch_few<SCN_DTYPE_FP32, 1>(p, stream);
-  else if (io.m <= 16) launch_few<SCN_DTYPE_MXFP4, 1>(p, stream);
+  int rc;
+  if (at == SCN_DTYPE_FP16) rc = launch_few<SCN_DTYPE_FP16, 1>(p, stream);
+  else if (at == SCN_DTYPE_FP32) rc = launch_few<SCN_DTYPE_FP32, 1>(p, stream);
+  else if (io.m <= 16) rc = launch_few<SCN_DTYPE_MXFP4, 1>(p, stream);
   // two row tiles of 16 where the tiled kernel below would run few workgroups down a long k: 32 rows, 1024 x 1024 weights 3.5
   // against 4.0 us, 4096 x 16384 24.5 against 36.6; but 8192 x 8192 24.6 against 20.3, 256 x 128 4.1 against 3.1
-  else if (io.m <= 32 && kb >= 32 && io.n <= 4096) launch_few<SCN_DTYPE_MXFP4, 2>(p, stream);
+  else if (io.m <= 32 && kb >= 32 && io.n <= 4096) rc = launch_few<SCN_DTYPE_MXFP4, 2>(p, stream);
   else {
     // The largest tile of which there are enough for the GPU's 256 CUs, when k is long enough for its reuse to count.  us for
     // 64 | 128 | 256 rows and channels a tile:
@@ -873,12 +881,12 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
     //   4096 x 64 x 8192 13.6 | 10.4, 16384 x 64 x 4096 (256 tiles) 12.8 | 10.0; x 2048 6.4 | 6.5; 24576 x 64 x 4096 14 | 17.
     const auto tiles = [&](uint32_t t) { return (uint64_t)ceil_div(io.n, t) * ceil_div(io.m, t); };
     const bool wide = kb > 16 || (io.res_dev && (uint64_t)io.m * io.n >= (16u << 20));
-    int rc = tiles(256) >= 144 && io.n > 128 && kb > 8 ? launch_product<256, 256, 4, 2, 1>(p, stream)
-             : tiles(128) >= 256 && io.n > 64 && wide  ? launch_product<128, 128, 2, 2, 1>(p, stream)
-             : tiles(64) <= 256 && kb > 120            ? launch_product<64, 64, 1, 1, 4>(p, stream)
-                                                       : launch_product<64, 64, 1, 1, 1>(p, stream);
-    if (rc) return rc;
+    rc = tiles(256) >= 144 && io.n > 128 && kb > 8 ? launch_product<256, 256, 4, 2, 1>(p, stream)
+         : tiles(128) >= 256 && io.n > 64 && wide  ? launch_product<128, 128, 2, 2, 1>(p, stream)
+         : tiles(64) <= 256 && kb > 120            ? launch_product<64, 64, 1, 1, 4>(p, stream)
+                                                   : launch_product<64, 64, 1, 1, 1>(p, stream);
   }
+  if (rc) return rc;
   SCN_HIP(hipGetLastError());
   return SCN_OK;
 }

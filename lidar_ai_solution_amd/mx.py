@@ -23,6 +23,7 @@ from .scn import _stream_ptr
 _DTYPE = {torch.float16: capi.DTYPE_FP16, torch.float32: capi.DTYPE_FP32, torch.int8: capi.DTYPE_INT8}
 _FLOATS = (torch.float16, torch.float32)
 _ROWS = (torch.float16, torch.float32, torch.int8)
+_COUNT = 1 << 32        # rows and strides are 32-bit numbers in the C ABI
 _L = None
 
 
@@ -48,6 +49,8 @@ def _using(stream, index: int):
     to the stream that its kernels run on."""
     if not isinstance(stream, torch.cuda.Stream):
         stream = torch.cuda.ExternalStream(int(stream), device=index) if int(stream) else torch.cuda.default_stream(index)
+    elif stream.device_index != index:
+        raise ValueError(f"a stream of cuda:{stream.device_index} for rows on cuda:{index}")
     return torch.cuda.stream(stream)
 
 
@@ -63,14 +66,16 @@ class MxRows:
     __slots__ = ("_codes", "_scales", "_buffer", "channels", "num_rows", "index", "codes_ptr", "codes_ld", "scales_ptr", "scales_ld")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, channels: int):
-        if channels < 1:
-            raise ValueError("rows need at least one channel")
+        if not 1 <= channels <= 1 << 30:
+            raise ValueError("rows need 1 to 2^30 channels")
         blocks = (channels + 31) // 32
         for t, need in ((codes, 16 * blocks), (scales, (blocks + 3) // 4 * 4)):
             if t.dtype != torch.uint8 or t.dim() != 2 or not t.is_cuda:
                 raise ValueError("codes and scales must be 2-D uint8 device tensors")
             if t.shape[1] < need or t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < need):
                 raise ValueError(f"rows of {channels} channels need {need} contiguous bytes of their own")
+        if codes.shape[0] >= _COUNT or max(_ld(codes), _ld(scales)) >= _COUNT:
+            raise ValueError("rows must be fewer than 2^32, less than 2^32 bytes apart")
         if codes.shape[0] != scales.shape[0] or codes.device != scales.device:
             raise ValueError("codes and scales must have the same rows on the same device")
         self._codes, self._scales, self._buffer = codes, scales, None
@@ -81,8 +86,8 @@ class MxRows:
     @classmethod
     def empty(cls, n: int, channels: int, device="cuda") -> "MxRows":
         """Uninitialised rows in the one-buffer form."""
-        if channels < 1 or n < 0:
-            raise ValueError("rows need at least one channel")
+        if not 1 <= channels <= 1 << 30 or not 0 <= n < _COUNT:
+            raise ValueError("rows need 1 to 2^30 channels, and are fewer than 2^32")
         self = cls.__new__(cls)
         blocks = (channels + 31) // 32
         size = (16 * blocks + (blocks + 3) // 4 * 4 + 15) // 16 * 16      # row_bytes(channels)
@@ -125,7 +130,11 @@ def _check_rows(x: torch.Tensor, dtypes, what: str) -> int:
         raise ValueError(f"{what} must have unit stride inside a row")
     if n > 1 and ld < c:
         raise ValueError(f"{what} must not have overlapping rows")
-    return ld if n > 1 else max(ld, c)
+    if n <= 1:
+        ld = max(ld, c)
+    if n >= _COUNT or ld >= _COUNT:
+        raise ValueError(f"{what} must have fewer than 2^32 rows, less than 2^32 elements apart")
+    return ld
 
 
 def _ld(x: torch.Tensor) -> int:
@@ -268,19 +277,23 @@ def product(a, b: MxRows, bias: Optional[torch.Tensor] = None, relu: bool = Fals
 
 
 class Rulebook:
-    """scn_rulebook: the neighbour table of a convolution (built once per set of coordinates, shared by its layers)."""
+    """scn_rulebook: the neighbour table of a convolution (built once per set of coordinates, shared by its layers).  It
+    lives on the device that is current when it is made."""
 
     def __init__(self, max_in: int, max_out: int, kernel_volume: int):
         self._h = capi.lib().scn_rulebook_create(max_in, max_out, kernel_volume)
         if not self._h:
             raise RuntimeError("rulebook creation failed: " + capi.lib().scn_last_error().decode())
         self._keep = None
+        self.index = _current_device()
         self.max_in, self.max_out = int(max_in), int(max_out)
         self.rows_in = self.rows_out = None   # bounds of the last build: rows the convolution may read / write
 
     def _check(self, indices: torch.Tensor):
         if indices.dtype != torch.int32 or indices.dim() != 2 or indices.shape[1] != 4 or not indices.is_contiguous() or not indices.is_cuda:
             raise ValueError("indices must be a contiguous int32 device tensor [n, 4]")
+        if not indices.get_device() == self.index == _current_device():
+            raise ValueError(f"the rulebook lives on cuda:{self.index}: indices and the current device must be that one")
 
     def build_subm(self, indices: torch.Tensor, grid: Sequence[int], kernel_size, dilation=(1, 1, 1), num=None, stream=None):
         self._check(indices)
@@ -311,7 +324,7 @@ class Rulebook:
 
 class Conv:
     """A sparse convolution on microscaled rows: weight fp16 [Cout, K0, K1, K2, Cin], bias fp16 [Cout] or None (host
-    arrays); both are laid out once."""
+    arrays); both are laid out once, on the device that is current then."""
 
     def __init__(self, weight: np.ndarray, bias: Optional[np.ndarray] = None):
         w = np.ascontiguousarray(weight, np.float16)
@@ -324,7 +337,7 @@ class Conv:
                                              None if b is None else b.ctypes.data_as(C.c_void_p), capi.PRECISION_MXFP4)
         if not self._h:
             raise RuntimeError("convolution creation failed: " + capi.lib().scn_last_error().decode())
-        self.cout, self.cin = int(w.shape[0]), int(w.shape[4])
+        self.cout, self.cin, self.index = int(w.shape[0]), int(w.shape[4]), _current_device()
 
     def forward(self, x: MxRows, rulebook: Rulebook, max_rows: int, relu: bool = False, residual: Optional[torch.Tensor] = None,
                 relu_after_add: bool = False, out=None, stream=None):
@@ -337,6 +350,8 @@ class Conv:
             raise ValueError("the rulebook has not been built")
         if x.num_rows < rulebook.rows_in or max_rows < rulebook.rows_out:
             raise ValueError(f"the rulebook covers {rulebook.rows_in} input rows and up to {rulebook.rows_out} output rows")
+        if not x.index == rulebook.index == self.index:
+            raise ValueError(f"rows on cuda:{x.index}, rulebook on cuda:{rulebook.index}, weights on cuda:{self.index}")
         if x.channels != self.cin:
             raise ValueError(f"input rows have {x.channels} channels, the weight expects {self.cin}")
         to_mx = isinstance(out, MxRows)

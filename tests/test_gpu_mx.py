@@ -148,6 +148,12 @@ def test_quantize_wrapper_refusals():
         mx.product(q, mx.quantize_rows(x[:, :32].contiguous()))
     with pytest.raises(ValueError):
         mx.product(q, q, bias=torch.zeros(3, device=DEV))
+    with pytest.raises(ValueError):
+        mx.quantize_rows(torch.empty_strided((1, 4), (1 << 32, 1), dtype=torch.float16, device=DEV))   # stride beyond 32 bits
+    with pytest.raises(RuntimeError):
+        mx.product(x, mx.quantize_rows(torch.zeros((64, 64), dtype=torch.float16, device=DEV)), out=x)
+    with pytest.raises(ValueError):
+        mx.MxRows.empty(-1, 4)
 
 
 # ------------------------------------------------------------------------------------------------- dequantise
@@ -511,6 +517,15 @@ def test_convolution_refusals():
         wide.forward(mx.quantize_rows(torch.zeros((50, 160), dtype=torch.float16, device=DEV)), rb, n_out, out=mx.MxRows.empty(n_out, 32, DEV))
     with pytest.raises(ValueError):
         conv.forward(q, rb, n_out, out=mx.MxRows.empty(n_out, 64, DEV))
+    same = mx.Conv(np.zeros((64, 3, 3, 3, 64), np.float16))
+    with pytest.raises(RuntimeError):                                     # in place
+        same.forward(q, rb, n_out, out=q)
+    rb.index, there = rb.index + 1, rb.index                              # (a rulebook of another device)
+    with pytest.raises(ValueError):
+        conv.forward(q, rb, n_out)
+    with pytest.raises(ValueError):
+        rb.build_subm(torch.zeros((5, 4), dtype=torch.int32, device=DEV), (9, 24, 21), (3, 3, 3))
+    rb.index = there
     with pytest.raises(RuntimeError):                                     # kernel volume
         mx.Conv(np.zeros((32, 1, 1, 1, 64), np.float16)).forward(q, rb, n_out)
 

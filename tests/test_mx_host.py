@@ -79,7 +79,7 @@ def test_dequantize_refusals(over):
 def _io(**over):
     io = capi.MxProductIO()
     base = dict(a_dev=GOOD, a_dtype=capi.DTYPE_MXFP4, a_ld=32, a_scales_dev=GOOD, a_scales_ld=4, b_codes_dev=GOOD, b_codes_ld=32,
-                b_scales_dev=GOOD, b_scales_ld=4, m=40, n=24, k=64, out_dev=GOOD, out_dtype=capi.DTYPE_FP16, out_ld=24)
+                b_scales_dev=GOOD, b_scales_ld=4, m=40, n=24, k=64, out_dev=GOOD + 4096, out_dtype=capi.DTYPE_FP16, out_ld=24)
     base.update(over)
     for key, v in base.items():
         setattr(io, key, v)
@@ -95,6 +95,21 @@ def _io(**over):
                                   dict(a_dtype=capi.DTYPE_FP32, a_ld=64, workspace_dev=GOOD + 8, workspace_bytes=1 << 20)])
 def test_product_refusals(over):
     assert capi.lib().scn_mx_product(C.byref(_io(**over)), None) == 1
+    assert b"mx_product" in capi.lib().scn_last_error()
+
+
+@pytest.mark.parametrize("over", [dict(out_dev=GOOD), dict(out_dev=GOOD, a_dtype=capi.DTYPE_FP16, a_ld=64, m=3),
+                                  dict(res_dev=GOOD + 4096, res_dtype=capi.DTYPE_FP16, res_ld=32),
+                                  dict(res_dev=GOOD + 4096, res_dtype=capi.DTYPE_FP32, res_ld=24)])
+def test_product_refuses_an_output_over_its_operands(over):
+    assert capi.lib().scn_mx_product(C.byref(_io(**over)), None) == 1
+    assert b"output" in capi.lib().scn_last_error()
+
+
+@pytest.mark.parametrize("over", [dict(m=1 << 31, n=64, out_ld=64), dict(m=1, n=1 << 27, out_ld=1 << 27), dict(m=17, n=0xFFFFFFFF, out_ld=0xFFFFFFFF),
+                                  dict(m=100, k=1 << 25, a_ld=1 << 25, b_codes_ld=1 << 25, a_scales_ld=1 << 25, b_scales_ld=1 << 25)])
+def test_product_refuses_what_one_launch_cannot_hold(over):
+    assert capi.lib().scn_mx_product(C.byref(_io(**over)), None) == 4          # SCN_ERR_UNSUPPORTED
     assert b"mx_product" in capi.lib().scn_last_error()
 
 
