@@ -78,7 +78,11 @@ __global__ __launch_bounds__(256) void k_conv_mx_rows(const ConvArgs a, const ui
 // kernel offsets out between them, so a wave only ever waits for its own loads; the waves' sums are added (in wave order) when
 // the rows are stored.
 //   a stage = one kernel offset that some row has a neighbour at (two of them for rows of one block): 64 gathered rows in LDS and
-//   the weights of its blocks in registers (in LDS they leave room for fewer waves); a wave fetches one stage ahead.  Rows without a neighbour fetch zeros (scale 2^-127, codes 0).
+//   the weights of its blocks in registers (in LDS they leave room for fewer waves); a wave fetches one stage ahead.  Rows without a
+//   neighbour read as zeros (scale 2^-127, codes 0).
+// (120,000 rows 64 -> 64, 21.6 us: 4.9 for the launch and the neighbour indices, 4.4 for the store, both near the memory's rate;
+// in between 5.9 for the products alone, 4.8 of gathers and 3 of weights on top.  Requesting the rows two stages ahead gains
+// 0.6 us here and loses 2 us at 60,000 rows 128 -> 128.)
 //   LDS rows of 3 and 5 chunks are read without bank conflicts as they are; rows of 2 and 4 chunks hold chunk c at position
 //   c ^ (row / 8) % 2 and c ^ (row / 4) % 4.
 template <int BPR, int MT, int W>
@@ -98,6 +102,11 @@ struct ConvMxStage {
 // reads behind every such load in flight.  m0 has no other user in this kernel.
 __device__ __forceinline__ void conv_load16_lds(const void* src, uint32_t base) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(base) : "memory");
+}
+
+// The same of a buffer: bytes [at, at + 16) of it, zeros beyond its size.
+__device__ __forceinline__ void conv_load16_lds(const v4i& buffer, uint32_t at, uint32_t base) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(at), "s"(buffer), "s"(base) : "memory");
 }
 
 // MODE: the epilogue (see epilogue_values): 2 and 4 are fp16 output without and with an fp16 residual, 0 everything.
@@ -143,6 +152,13 @@ __global__ __launch_bounds__(64 * W, 2) void k_conv_mx_gather(const ConvArgs a, 
     woff[s] = (b * mtiles + t0) * 32 + ln;
     soff[s] = (b * ((mtiles + 3) / 4) + t0 / 4) * 32 + ln;
   }
+  // The input rows as a buffer of 2^24 - 1 of them, where the table can name no more and they fit 32 bits: "no neighbour" (-1,
+  // 2^24 - 1 in the 24 bits that the multiplication takes) lies behind its end, where loads return 0.  An address is one
+  // instruction then (120,000 rows 64 -> 64: 22.9 us with 64-bit addresses and a row of zeros, 21.5 us so).
+  const bool near = a.nbr_ld < (1u << 24) && a.x_ld_bytes < 256;
+  const uint64_t xbase = (uint64_t)(uintptr_t)a.x;
+  const v4i xbuf = {__builtin_amdgcn_readfirstlane((int)(uint32_t)xbase), __builtin_amdgcn_readfirstlane((int)(uint32_t)(xbase >> 32) & 0xFFFF),
+                    (int)(0xFFFFFFu * a.x_ld_bytes), 0x00027000};
   uint4 w[S::KS][MT], w1[S::KS][MT];
   uint32_t ws[S::KS], ws1[S::KS];
 
@@ -205,11 +221,19 @@ __global__ __launch_bounds__(64 * W, 2) void k_conv_mx_gather(const ConvArgs a, 
           w1[s][t] = *reinterpret_cast<const uint4*>(wp + (woff[s] + other * wstride + min(t, mtiles - 1 - t0) * 32) * 16);
         ws1[s] = *reinterpret_cast<const uint32_t*>(sp + (soff[s] + other * sstride) * 4);
       }
+      if (near) {
 #pragma unroll
-      for (int q = 0; q < S::GLOADS; ++q) {
-        const char* row = a.x + (size_t)(uint32_t)max(i[q], 0) * a.x_ld_bytes;
-        row = i[q] >= 0 && (q < S::CH || second) ? row : a.zrow;
-        conv_load16_lds(row + gchunk[q % S::CH], buf + q * 1024);
+        for (int q = 0; q < S::GLOADS; ++q) {
+          const uint32_t at = ((uint32_t)i[q] & 0xFFFFFFu) * (a.x_ld_bytes & 0xFFFFFFu) + gchunk[q % S::CH];
+          conv_load16_lds(xbuf, q < S::CH || second ? at : 0xFFFFFFF0u, buf + q * 1024);
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < S::GLOADS; ++q) {
+          const char* row = a.x + (size_t)(uint32_t)max(i[q], 0) * a.x_ld_bytes;
+          row = i[q] >= 0 && (q < S::CH || second) ? row : a.zrow;
+          conv_load16_lds(row + gchunk[q % S::CH], buf + q * 1024);
+        }
       }
     };
     if (stages > 0) issue(0);
@@ -345,9 +369,9 @@ static void launch_gather(ConvArgs& a, const uint8_t* ws, int mtiles, hipStream_
 
 // Waves per 64 rows.  Few tiles are bound by the latency of a wave's chain of stages, which more waves shorten; where the tiles
 // of one wave just fill the GPU (12 per CU), one has the fewest instructions; beyond that two balance better.  us with 1 / 2 / 4
-// waves: 20,000 rows 64 -> 64 14.1 / 10.9 / 8.2, 120,000 rows 22.9 / 26.6 / 25.9, 260,000 rows 45.7 / 41.1 / 45.4; with 128
-// output channels (twice the work per wave) 20,000 rows 128 -> 128 26.3 / 20.1 / 15.9, 48,460 rows 64 -> 128 20.8 / 17.2 / 19.1,
-// 150,000 rows 128 -> 128 68.1 / 60.0 / 63.0.
+// waves: 20,000 rows 64 -> 64 14.2 / 10.2 / 7.9, 120,000 rows 22.2 / 25.4 / 25.3, 260,000 rows 45.0 / 40.5 / 45.1; with 128
+// output channels (twice the work per wave) with 2 / 4: 20,000 rows 128 -> 128 18.6 / 15.5, 48,460 rows 64 -> 128 15.8 / 18.9,
+// 150,000 rows 128 -> 128 59.3 / 61.7.
 // The choice follows the bound of the row count, never the count or what an earlier forward had: the order of the sums, and
 // so their last bit, depends on it.
 template <int BPR, int MODE>

@@ -467,6 +467,22 @@ def test_convolution_stores_microscaled_rows(cin, cout, n, ks, stride, pad, subm
         assert (got.codes[n_out:] == 0xAA).all() and (got.scales[n_out:] == 0xBB).all()
 
 
+@pytest.mark.parametrize("cin, ld", [(16, 256), (64, 272), (96, 4096), (128, 256), (160, 65536), (64, 1 << 22)])
+def test_convolution_of_rows_far_apart(cin, ld):
+    """The last one spans 4.8 GB."""
+    mx = _mx()
+    rng = np.random.default_rng(cin + ld)
+    rb, _, n_out, conv, _, _ = conv_case(rng, 1200, (9, 24, 21), cin, 48, (3, 3, 3), (1, 1, 1), (1, 1, 1), True)
+    q = mx.quantize_rows(torch.from_numpy(rows(rng, 1200, cin)).to(DEV))
+    b = 16 * ((cin + 31) // 32)
+    big = torch.empty((1200, ld), dtype=torch.uint8, device=DEV)
+    big[:, :b], big[:, b:b + q.scales.shape[1]] = q.codes, q.scales
+    if ld < 1 << 20:
+        big[:, b + q.scales.shape[1]:] = 0xFF
+    far = mx.MxRows(big[:, :b], big[:, b:b + q.scales.shape[1]], cin)
+    assert torch.equal(conv.forward(far, rb, n_out), conv.forward(q, rb, n_out))
+
+
 def test_convolution_nan_rows_reach_their_neighbours_only():
     mx = _mx()
     rng = np.random.default_rng(3)
