@@ -113,7 +113,7 @@ _SIGNATURES = {
     "scn_mx_row_bytes": (C.c_size_t, [u32]),
     "scn_mx_quantize_rows": (C.c_int, [vp, C.c_int, u32, u32, C.c_float, C.c_int, vp, u32, vp, u32, u32, vp, vp]),
     "scn_mx_dequantize_rows": (C.c_int, [vp, u32, vp, u32, u32, vp, C.c_int, u32, u32, vp, vp]),
-    "scn_mx_product_workspace": (C.c_size_t, [u32, u32]),
+    "scn_mx_product_workspace": (C.c_size_t, [u32, u32, u32]),
     "scn_mx_product": (C.c_int, [vp, vp]),
     "scn_scatter_dense": (C.c_int, [vp, C.c_int, C.c_float, u32, u32, vp, u32, vp, i5, vp, vp, vp]),
     "scn_scatter_dense_layout": (C.c_int, [vp, C.c_int, C.c_float, u32, u32, vp, u32, vp, i5, vp, C.c_int, C.c_int,

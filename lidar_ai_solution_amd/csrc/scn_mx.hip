@@ -778,11 +778,186 @@ static int launch_product(const ProductArgs& p, hipStream_t stream) {
   return SCN_OK;
 }
 
+// Rows that are not quantised yet, of up to P blocks (P = 2, 4 or 8), times up to a few hundred channels: bound by the rows, the
+// residual and the output.  A workgroup owns BM rows x 64 WN channels, a wave TM tiles of 32 rows x 64 channels.  Everything it
+// reads is requested at the start: the weights straight to LDS (see above for the order of their blocks), the rows and the
+// residual to registers; the rows are quantised into LDS in the operands' order, and one barrier later multiplied.
+// (123,646 x 256 x 128, fp16 rows and residual: 34.9 us, 4.5 TB/s of what it cannot do without.)
+template <int AT, int WN, int P>
+struct FusedTile {
+  // 8 waves share the quantisation of long rows; where the tile has fewer outputs than waves, the others do no more
+  static constexpr int NW = P == 8 ? 8 : 4, WM = P == 8 ? 2 : 4 / WN, TM = P == 8 || WN < 4 ? 1 : 2, BM = 32 * TM * WM;
+  static constexpr int XS = BM * P * 16, WC = XS + BM * 8;           // LDS offsets: codes of the rows, their scales, weights
+  static constexpr int PAD = 68, STORE = WN * WM * 32 * PAD * 4;       // floats per row of the store buffer, its bytes
+  static constexpr int LDS = WC + WN * 64 * P * 16 > STORE ? WC + WN * 64 * P * 16 : STORE;
+};
+
+template <int AT, int WN, int P>
+__global__ __launch_bounds__((64 * FusedTile<AT, WN, P>::NW)) void k_mx_product_fused(const ProductArgs p) {
+  using F = FusedTile<AT, WN, P>;
+  typedef typename MxIn<AT>::T T;
+  constexpr int TM = F::TM, BM = F::BM, NW = F::NW, E = 16 / (int)sizeof(T), LPB = 32 / E, WORDS = (P + 3) / 4;
+  __shared__ __align__(16) char lds[F::LDS];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = lane & 31, lh = lane >> 5;
+  const int wn = wave % WN, wm = wave / WN;
+  const uint32_t m = eff_n(p.m_dev, p.m);
+  const uint32_t i0 = blockIdx.x * BM, n0 = blockIdx.y * 64 * WN;
+  if (i0 >= m) return;
+  const uint32_t last_w = p.n - 1 - n0;
+  auto swizzle = [](uint32_t row) { return row / (16 / P) % P; };
+
+  const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(mx_lptr)lds);
+  const uint8_t* wcode = p.b + (size_t)n0 * p.b_ld;
+#pragma unroll
+  for (int u = 0; u < (WN * P + NW - 1) / NW; ++u) {
+    const int unit = u * NW + wave;
+    if (unit < WN * P) {   // 64 of the P * 64 * WN chunks of weights
+      const uint32_t e = unit * 64 + lane, r = e / P, blk = (e % P) ^ swizzle(r);
+      mx_load16_lds(wcode, min(r, last_w) * p.b_ld + (blk < p.kb ? blk * 16 : 0u), base + F::WC + unit * 1024);
+    }
+  }
+  uint32_t ws[2][WORDS];
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int q = 0; q < WORDS; ++q) {
+      const uint8_t* row = p.bs + (size_t)(n0 + min((uint32_t)(wn * 64 + a * 32 + ln), last_w)) * p.bs_ld;
+      const uint32_t left = p.kb > 4u * q ? p.kb - 4 * q : 0u;
+      ws[a][q] = left ? *reinterpret_cast<const uint32_t*>(row + 4 * q) & (left >= 4 ? ~0u : (1u << (8 * left)) - 1u) : 0u;
+    }
+  constexpr int LPR = 8, RPP = 8, PASSES = 4;   // lanes per row (8 channels each), rows per pass, passes per 32 rows
+  const uint32_t row0 = i0 + wm * 32 * TM + lane / LPR, ch = n0 + wn * 64 + (lane % LPR) * 8;
+  v4u pre[TM * PASSES];
+  const bool works = wave < WN * F::WM, want = works && p.res && !p.res_fp32 && ch + 8 <= p.n;
+#pragma unroll
+  for (int q = 0; q < TM * PASSES; ++q) {
+    pre[q] = v4u{0, 0, 0, 0};
+    const uint32_t row = row0 + q * RPP;
+    if (want && row < m) __builtin_memcpy(&pre[q], (const _Float16*)p.res + (size_t)row * p.res_ld + ch, 16);
+  }
+
+  constexpr int PIECES = BM * P * LPB / (64 * NW), BATCH = PIECES < 16 ? PIECES : 16;   // pieces of 16 bytes per thread
+#pragma unroll 1
+  for (int i = 0; i < PIECES; i += BATCH) {
+    // whole pieces are requested all at once (other lanes read the tile's first one); a row's last one, if it is short, later
+    T raw[BATCH][E];
+    if (p.k >= (uint32_t)E) {
+#pragma unroll
+      for (int z = 0; z < BATCH; ++z) {
+        const uint32_t e = (i + z) * 64 * NW + threadIdx.x, at = e / LPB % P * 32 + e % LPB * E, row = i0 + e / (LPB * P);
+        const bool whole = at + E <= p.k && row < m;
+        __builtin_memcpy(raw[z], (const T*)p.a + (whole ? (size_t)row * p.a_ld + at : (size_t)i0 * p.a_ld), 16);
+      }
+    }
+#pragma unroll
+    for (int z = 0; z < BATCH; ++z) {
+      const uint32_t e = (i + z) * 64 * NW + threadIdx.x, sub = e % LPB, blk = e / LPB % P, row = e / (LPB * P), at = blk * 32 + sub * E;
+      const bool whole = at + E <= p.k && i0 + row < m;
+      float v[E];
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = whole ? (float)raw[z][j] : 0.f;
+      if (!whole && at < p.k && i0 + row < m) mx_load<AT, E>((const T*)p.a + (size_t)(i0 + row) * p.a_ld, at, p.k, 1.f, 0, v);
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < E; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+      top = lanes_max<LPB>(top);
+      const uint32_t sc = mx_scale_byte(top);
+      const float up = __uint_as_float((254u - (sc == 255u ? 0u : sc)) << 23);
+      char* dst = lds + (row * P + (blk ^ swizzle(row))) * 16 + sub * (E / 2);
+      if constexpr (E == 8) {
+        *reinterpret_cast<uint32_t*>(dst) = sc == 255u ? 0u : mx_codes8(v, up);
+      } else {
+        uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[0] * up, v[1] * up, 1.f, 0);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2] * up, v[3] * up, 1.f, 1);
+        *reinterpret_cast<uint16_t*>(dst) = sc == 255u ? (uint16_t)0 : (uint16_t)w;
+      }
+      if (sub == 0) *reinterpret_cast<uint8_t*>(lds + F::XS + row * 8 + blk) = blk < p.kb ? (uint8_t)sc : (uint8_t)0;
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // (the weights too)
+  __syncthreads();
+
+  v16f acc[2][TM];
+  if (works) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int b = 0; b < TM; ++b)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[a][b][j] = 0.f;
+#pragma unroll
+    for (int s = 0; s < P / 2; ++s) {   // 64 channels; blocks that do not exist have scales of 2^-127 on both sides
+      const uint32_t pos = ((2 * s + lh) ^ swizzle(ln)) * 16;
+      v4i w[2], x[TM];
+      uint32_t xs[TM];
+#pragma unroll
+      for (int a = 0; a < 2; ++a) w[a] = *reinterpret_cast<const v4i*>(lds + F::WC + (wn * 64 + a * 32 + ln) * P * 16 + pos);
+#pragma unroll
+      for (int b = 0; b < TM; ++b) {
+        const uint32_t row = (wm * TM + b) * 32 + ln;
+        x[b] = *reinterpret_cast<const v4i*>(lds + row * P * 16 + pos);
+        xs[b] = *reinterpret_cast<const uint32_t*>(lds + F::XS + row * 8 + s / 2 * 4) >> (8 * lh);
+      }
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < TM; ++b)
+          acc[a][b] = s & 1 ? mx_mma32_sel<2>(w[a], ws[a][s / 2] >> (8 * lh), x[b], xs[b], acc[a][b])
+                            : mx_mma32_sel<0>(w[a], ws[a][s / 2] >> (8 * lh), x[b], xs[b], acc[a][b]);
+    }
+  }
+  __syncthreads();
+  if (!works) return;
+  // store through LDS as above
+  float* buf = reinterpret_cast<float*>(lds) + wave * 32 * F::PAD;
+#pragma unroll
+  for (int b = 0; b < TM; ++b) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<v4f*>(buf + ln * F::PAD + a * 32 + q * 8 + lh * 4) =
+            v4f{acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]};
+#pragma unroll
+    for (int r = 0; r < PASSES; ++r) {
+      const uint32_t row = row0 + (b * PASSES + r) * RPP;
+      if (row < m && ch < p.n) product_store8(p, row, ch, buf + (r * RPP + lane / LPR) * F::PAD + (lane % LPR) * 8, pre[b * PASSES + r]);
+    }
+  }
+}
+
+template <int AT, int WN>
+static void launch_fused(const ProductArgs& p, hipStream_t stream) {
+  const auto launch = [&](auto kernel, uint32_t rows, uint32_t waves) {
+    hipLaunchKernelGGL(kernel, dim3(ceil_div(p.m, rows), ceil_div(p.n, 64u * WN)), dim3(64 * waves), 0, stream, p);
+  };
+  if (p.kb <= 2) launch(k_mx_product_fused<AT, WN, 2>, FusedTile<AT, WN, 2>::BM, FusedTile<AT, WN, 2>::NW);
+  else if (p.kb <= 4) launch(k_mx_product_fused<AT, WN, 4>, FusedTile<AT, WN, 4>::BM, FusedTile<AT, WN, 4>::NW);
+  else launch(k_mx_product_fused<AT, WN, 8>, FusedTile<AT, WN, 8>::BM, FusedTile<AT, WN, 8>::NW);
+}
+template <int AT>
+static int launch_fused(const ProductArgs& p, hipStream_t stream) {
+  SCN_REQUIRE((uint64_t)p.b_ld * 256 < (1ull << 32), SCN_ERR_UNSUPPORTED, "mx_product: rows more than 16 MB apart");
+  if (p.n <= 64) launch_fused<AT, 1>(p, stream);
+  else if (p.n <= 128) launch_fused<AT, 2>(p, stream);
+  else launch_fused<AT, 4>(p, stream);
+  return SCN_OK;
+}
+
 // Rows that are not quantised yet are quantised by every workgroup that reads them up to this many blocks; beyond it (and
 // beyond 16 rows) a launch of its own is cheaper: 8192 x 8192 weights, 4 fp16 rows (1024 blocks): 15.4 us against 15.8 us,
 // 8 rows 19.9 us against 17.3 us.
 static bool product_direct(uint32_t m, uint32_t k) { return m <= 16 && (uint64_t)m * mx_blocks(k) <= kFewBlocks; }
-static size_t product_workspace(uint32_t m, uint32_t k) { return product_direct(m, k) ? 0 : (size_t)m * mx_row_bytes(k); }
+// More of them are quantised in the product's own launch while their channels are few: every workgroup of a row quantises it, one
+// for 256 channels.  us with the two launches | one, fp16 rows: 123646 x 256 x 128 with residual 41.5 | 34.9, 123646 x 64 x 64 14.1 |
+// 8.7, 50000 x 1024 x 64 29.5 | 27.8, 20000 x 1000 x 100 27.6 | 24.6, 50000 x 256 x 256 19.6 | 19.7 (fp32 30.5 | 25.0), 500 x 64 x 256
+// 5.4 | 5.2; but 50000 x 512 x 256 23.6 | 25.7, 5000 x 1024 x 256 8.0 | 9.4.  One launch is 6 us less on the host.
+static bool product_fused(uint32_t m, uint32_t n, uint32_t k) {
+  return m < (1u << 29) && (k <= 128 ? n <= 1024 : k <= 256 && n <= 256);
+}
+static size_t product_workspace(uint32_t m, uint32_t n, uint32_t k) {
+  return product_direct(m, k) || product_fused(m, n, k) ? 0 : (size_t)m * mx_row_bytes(k);
+}
 
 // U = runs a wave requests at once: what it has to do in all, up to 8 (4 for two row tiles).
 template <int AT, int MT>
@@ -849,8 +1024,8 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
   } else {
     SCN_REQUIRE(io.a_dev && aligned(io.a_dev, at) && io.a_ld >= io.k, SCN_ERR_INVALID,
                 "mx_product: null or misaligned rows, or row stride %u < %u channels", io.a_ld, io.k);
-    if (!product_direct(io.m, io.k)) {
-      const size_t need = product_workspace(io.m, io.k);
+    if (!product_direct(io.m, io.k) && !product_fused(io.m, io.n, io.k)) {
+      const size_t need = product_workspace(io.m, io.n, io.k);
       SCN_REQUIRE(io.workspace_dev && ((uintptr_t)io.workspace_dev & 15) == 0 && io.workspace_bytes >= need, SCN_ERR_INVALID,
                   "mx_product: rows of this type need a 16-byte aligned workspace of %zu bytes (%zu given)", need, io.workspace_bytes);
       uint8_t* ws = (uint8_t*)io.workspace_dev;
@@ -864,7 +1039,9 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
     }
   }
   int rc;
-  if (at == SCN_DTYPE_FP16) rc = launch_few<SCN_DTYPE_FP16, 1>(p, stream);
+  if (at != SCN_DTYPE_MXFP4 && !product_direct(io.m, io.k))
+    rc = at == SCN_DTYPE_FP16 ? launch_fused<SCN_DTYPE_FP16>(p, stream) : launch_fused<SCN_DTYPE_FP32>(p, stream);
+  else if (at == SCN_DTYPE_FP16) rc = launch_few<SCN_DTYPE_FP16, 1>(p, stream);
   else if (at == SCN_DTYPE_FP32) rc = launch_few<SCN_DTYPE_FP32, 1>(p, stream);
   else if (io.m <= 16) rc = launch_few<SCN_DTYPE_MXFP4, 1>(p, stream);
   // two row tiles of 16 where the tiled kernel below would run few workgroups down a long k: 32 rows, 1024 x 1024 weights 3.5
@@ -917,7 +1094,7 @@ int scn_mx_dequantize_rows(const uint8_t* codes_dev, uint32_t codes_ld, const ui
   return rc;
 }
 
-size_t scn_mx_product_workspace(uint32_t m, uint32_t k) { return k ? product_workspace(m, k) : 0; }
+size_t scn_mx_product_workspace(uint32_t m, uint32_t n, uint32_t k) { return k ? product_workspace(m, n, k) : 0; }
 
 int scn_mx_product(const scn_mx_product_io* io, void* stream) {
   SCN_REQUIRE(io, SCN_ERR_INVALID, "scn_mx_product: null pointer");

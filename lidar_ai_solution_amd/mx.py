@@ -247,7 +247,7 @@ def product(a, b: MxRows, bias: Optional[torch.Tensor] = None, relu: bool = Fals
         (m, k), a_index = a.shape, a.get_device()
         a_ptr, a_dtype, as_ptr, as_ld = a.data_ptr(), _DTYPE[a.dtype], 0, 0
         if workspace is None:
-            ws_bytes = L.scn_mx_product_workspace(m, k)
+            ws_bytes = L.scn_mx_product_workspace(m, n, k)
             if ws_bytes:
                 workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=_device(index))
         if workspace is not None:

@@ -256,6 +256,34 @@ def test_products_down_a_long_k(m, n, k, res_dtype):
         assert torch.equal(again, out)
 
 
+# quantised in the product's launch (k up to 128 with n up to 1024, up to 256 with n up to 256), and just beyond
+@pytest.mark.parametrize("m, n, k", [(70, 300, 1), (129, 65, 7), (200, 129, 33), (65, 1024, 127), (100, 1025, 128), (64, 256, 256), (63, 257, 256),
+                                     (1000, 255, 250), (90, 20, 200), (300, 64, 64), (260, 128, 9), (17, 70, 3), (5000, 100, 129), (33, 200, 257)])
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("res_dtype", [None, np.float16, np.float32])
+def test_product_of_short_rows(m, n, k, dtype, res_dtype):
+    mx = _mx()
+    rng = np.random.default_rng(m + n + k)
+    w, wv = mx_rows(rng, n, k)
+    w.scales[:, -(-k // 32):] = 255                                        # (padding: not read)
+    h = rows(rng, m, k, dtype)
+    a = strided(h, k + 3, 1)
+    bias = rng.standard_normal(n).astype(np.float32)
+    res = None if res_dtype is None else rng.standard_normal((m, n)).astype(res_dtype)
+    y, mag = R.product(R.fake(h), wv, bias, True, res, False)
+    for out_dtype, kept in ((torch.float16, m), (torch.float32, m - 5), (torch.float32, 0)):
+        out = strided(np.full((m, n), 9, NP[out_dtype]), n + 2, 1)
+        num = torch.tensor([kept], dtype=torch.int32, device=DEV)
+        mx.product(a, w, bias=torch.from_numpy(bias).to(DEV), relu=True, residual=None if res is None else strided(res, n + 1, 1), out=out, num=num)
+        got = out.double().cpu().numpy()
+        R.within(got[:kept], y[:kept], R.tolerance(y, mag, k, HALF[out_dtype])[:kept])
+        assert (got[kept:] == 9).all()
+    if res_dtype == np.float16:                                            # over its residual
+        t = torch.from_numpy(res).to(DEV)
+        mx.product(a, w, bias=torch.from_numpy(bias).to(DEV), relu=True, residual=t, out=t)
+        R.within(t.double().cpu().numpy(), y, R.tolerance(y, mag, k, 2.0 ** -11))
+
+
 @pytest.mark.parametrize("m", [5, 60, 400])
 def test_product_device_count_strides_and_untouched_memory(m):
     mx = _mx()

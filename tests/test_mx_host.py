@@ -41,8 +41,8 @@ def test_row_bytes():
     for c in range(1, 600):
         blocks = -(-c // 32)
         assert L.scn_mx_row_bytes(c) == -(-(16 * blocks + -(-blocks // 4) * 4) // 16) * 16
-    assert L.scn_mx_product_workspace(16, 64) == 0
-    assert L.scn_mx_product_workspace(17, 64) == 17 * L.scn_mx_row_bytes(64)
+    assert L.scn_mx_product_workspace(16, 5000, 64) == 0
+    assert L.scn_mx_product_workspace(17, 24, 257) == 17 * L.scn_mx_row_bytes(257)
 
 
 def _quantize(**over):
@@ -76,6 +76,9 @@ def test_dequantize_refusals(over):
     assert b"mx_dequantize_rows" in capi.lib().scn_last_error()
 
 
+LONG = dict(k=320, a_ld=320, b_codes_ld=160, b_scales_ld=12)      # rows that need a workspace (40 of 176 bytes)
+
+
 def _io(**over):
     io = capi.MxProductIO()
     base = dict(a_dev=GOOD, a_dtype=capi.DTYPE_MXFP4, a_ld=32, a_scales_dev=GOOD, a_scales_ld=4, b_codes_dev=GOOD, b_codes_ld=32,
@@ -91,8 +94,8 @@ def _io(**over):
                                   dict(out_dtype=capi.DTYPE_INT8), dict(out_ld=23), dict(bias_dev=GOOD, bias_dtype=capi.DTYPE_INT8),
                                   dict(bias_dev=GOOD + 2, bias_dtype=capi.DTYPE_FP32), dict(res_dev=GOOD, res_dtype=0),
                                   dict(res_dev=GOOD, res_dtype=capi.DTYPE_FP16, res_ld=23), dict(a_dtype=capi.DTYPE_FP16, a_ld=63),
-                                  dict(a_dtype=capi.DTYPE_FP16, a_ld=64), dict(a_dtype=capi.DTYPE_FP32, a_ld=64, workspace_dev=GOOD, workspace_bytes=1919),
-                                  dict(a_dtype=capi.DTYPE_FP32, a_ld=64, workspace_dev=GOOD + 8, workspace_bytes=1 << 20)])
+                                  dict(LONG, a_dtype=capi.DTYPE_FP16), dict(LONG, a_dtype=capi.DTYPE_FP32, workspace_dev=GOOD, workspace_bytes=7039),
+                                  dict(LONG, a_dtype=capi.DTYPE_FP32, workspace_dev=GOOD + 8, workspace_bytes=1 << 20)])
 def test_product_refusals(over):
     assert capi.lib().scn_mx_product(C.byref(_io(**over)), None) == 1
     assert b"mx_product" in capi.lib().scn_last_error()
