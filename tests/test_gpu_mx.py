@@ -1,4 +1,6 @@
 """Microscaled 4-bit rows on the GPU against their float64 oracle (tests/mx_reference.py)."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -493,6 +495,63 @@ def test_convolution_stores_microscaled_rows(cin, cout, n, ks, stride, pad, subm
         assert conv.forward(q, rb, n_out, out=got, **kw) is got
         assert torch.equal(got.codes[:n_out], want.codes) and torch.equal(got.scales[:n_out], want.scales)
         assert (got.codes[n_out:] == 0xAA).all() and (got.scales[n_out:] == 0xBB).all()
+
+
+@pytest.mark.parametrize("cin, cout, bound", [(16, 16, 500), (64, 64, 500), (64, 64, 40000), (96, 128, 500), (32, 48, 120000), (160, 32, 500)])
+@pytest.mark.parametrize("res", [None, "fp16", "int8", "requantised"])
+def test_convolution_int8_output_and_every_residual(cin, cout, bound, res):
+    """The epilogue's arithmetic on the sums that the kernel dumps, in fp32 step by step: bit for bit."""
+    mx = _mx()
+    f32 = np.float32
+    rng = np.random.default_rng(cin + cout)
+    coords = scene(rng, 500, (9, 24, 21))
+    idx = torch.zeros((bound, 4), dtype=torch.int32, device=DEV)
+    idx[:500, 1:] = torch.from_numpy(coords.astype(np.int32)).to(DEV)
+    rb = mx.Rulebook(bound, bound, 27)
+    rb.build_subm(idx, (9, 24, 21), (3, 3, 3), num=torch.tensor([500], dtype=torch.int32, device=DEV))
+    w = (rng.standard_normal((cout, 3, 3, 3, cin)) / np.sqrt(4 * cin)).astype(np.float16)
+    b = rng.standard_normal(cout).astype(np.float16)
+    conv = mx.Conv(w, b)
+    q = mx.quantize_rows(torch.from_numpy(rows(rng, 500, cin)).to(DEV))
+    r16, r8 = rng.standard_normal((500, cout)).astype(np.float16), rng.integers(-127, 128, (500, cout)).astype(np.int8)
+
+    def quant(y, amax):
+        return np.clip(np.rint(y * (f32(127) / f32(amax))), -127, 127).astype(f32)
+
+    def step(amax):
+        return f32(amax) / f32(127)
+
+    for relu in (0, 1):
+        acc = torch.full((500, cout), 7.0, device=DEV)
+        out = torch.full((503, cout), 9, dtype=torch.int8, device=DEV)
+        io = capi.ConvIO()
+        io.x_dev, io.x_ld, io.relu, io.out_dtype, io.out_dynamic_range = q.codes_ptr, q.codes_ld, relu, capi.DTYPE_INT8, 5.0
+        io.out_dev, io.out_ld, io.acc_dev = out.data_ptr(), cout, acc.data_ptr()
+        keep = None
+        if res is not None:
+            keep = torch.from_numpy(r8 if res == "int8" else r16).to(DEV)
+            io.res_dev, io.res_ld, io.relu_after_add = keep.data_ptr(), cout, 1 - relu
+            io.res_dtype = capi.DTYPE_INT8 if res == "int8" else capi.DTYPE_FP16
+            io.mid_dtype = io.res_dtype
+            if res == "int8":
+                io.res_dynamic_range, io.mid_dynamic_range = 3.0, 4.0
+            if res == "requantised":
+                io.a_requant_range, io.b_requant_range = 2.5, 3.5
+        capi.check(capi.lib().scn_conv_forward(conv._h, rb._h, C.byref(io), torch.cuda.current_stream().cuda_stream))
+        y = acc.cpu().numpy() + b.astype(f32)
+        if relu:
+            y = np.maximum(y, f32(0))
+        if res == "int8":
+            y = quant(y, 4.0) * step(4.0) + r8.astype(f32) * step(3.0)
+        elif res is not None:
+            y, r = y.astype(np.float16).astype(f32), r16.astype(f32)
+            if res == "requantised":
+                y, r = quant(y, 2.5) * step(2.5), quant(r, 3.5) * step(3.5)
+            y = y + r
+        if res is not None and not relu:
+            y = np.maximum(y, f32(0))
+        got = out.cpu().numpy()
+        assert np.array_equal(got[:500], quant(y, 5.0).astype(np.int8)) and (got[500:] == 9).all()
 
 
 @pytest.mark.parametrize("cin, ld", [(16, 256), (64, 272), (96, 4096), (128, 256), (160, 65536), (64, 1 << 22)])
