@@ -1038,15 +1038,21 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
       at = SCN_DTYPE_MXFP4;
     }
   }
+  const auto tiles = [&](uint32_t t) { return (uint64_t)ceil_div(io.n, t) * ceil_div(io.m, t); };
+  // Up to 16 rows, except where the tiles of the kernel that divides k between waves fill the GPU: it reads the rows once per 64
+  // channels, not per 16.  us few | tiled: 8192 x 8192 weights 1 row 11.0 | 11.9, 4 rows 13.0 | 12.0, 16 rows 17.1 | 12.2; 5000 x 8192 1
+  // row 11.0 | 11.4, 16 rows 17.0 | 12.1; 16384 x 4096 (256 tiles) 1 row 11.1 | 9.7; but 4096 x 16384 (64 tiles) 16 rows 17.1 | 20.1,
+  // 8192 x 2048 5.8 | 6.9
+  const bool few = io.m <= 16 && !(kb > 120 && tiles(64) >= (io.m > 2 ? 72u : 256u));
   int rc;
   if (at != SCN_DTYPE_MXFP4 && !product_direct(io.m, io.k))
     rc = at == SCN_DTYPE_FP16 ? launch_fused<SCN_DTYPE_FP16>(p, stream) : launch_fused<SCN_DTYPE_FP32>(p, stream);
   else if (at == SCN_DTYPE_FP16) rc = launch_few<SCN_DTYPE_FP16, 1>(p, stream);
   else if (at == SCN_DTYPE_FP32) rc = launch_few<SCN_DTYPE_FP32, 1>(p, stream);
-  else if (io.m <= 16) rc = launch_few<SCN_DTYPE_MXFP4, 1>(p, stream);
-  // two row tiles of 16 where the tiled kernel below would run few workgroups down a long k: 32 rows, 1024 x 1024 weights 3.5
-  // against 4.0 us, 4096 x 16384 24.5 against 36.6; but 8192 x 8192 24.6 against 20.3, 256 x 128 4.1 against 3.1
-  else if (io.m <= 32 && kb >= 32 && io.n <= 4096) rc = launch_few<SCN_DTYPE_MXFP4, 2>(p, stream);
+  else if (few) rc = launch_few<SCN_DTYPE_MXFP4, 1>(p, stream);
+  // two row tiles of 16 while the tiled kernel below does not divide k: 32 rows, 1024 x 1024 weights 3.5 against 4.0 us, 8192 x 2048
+  // 7.4 against 7.1
+  else if (io.m > 16 && io.m <= 32 && kb >= 32 && kb < 64 && io.n <= 4096) rc = launch_few<SCN_DTYPE_MXFP4, 2>(p, stream);
   else {
     // The largest tile of which there are enough for the GPU's 256 CUs, when k is long enough for its reuse to count.  us for
     // 64 | 128 | 256 rows and channels a tile:
@@ -1056,7 +1062,6 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
     //   123646 x 256 x 128 31 | 28 | 31, 50000 x 256 x 128 10.6 | 13.2 | 12.7.
     // The smallest tile with k in 4 parts, when there is a CU for every tile and 16 stages: whole | in 4 parts
     //   4096 x 64 x 8192 13.6 | 10.4, 16384 x 64 x 4096 (256 tiles) 12.8 | 10.0; x 2048 6.4 | 6.5; 24576 x 64 x 4096 14 | 17.
-    const auto tiles = [&](uint32_t t) { return (uint64_t)ceil_div(io.n, t) * ceil_div(io.m, t); };
     const bool wide = kb > 16 || (io.res_dev && (uint64_t)io.m * io.n >= (16u << 20));
     rc = tiles(256) >= 144 && io.n > 128 && kb > 8 ? launch_product<256, 256, 4, 2, 1>(p, stream)
          : tiles(128) >= 256 && io.n > 64 && wide  ? launch_product<128, 128, 2, 2, 1>(p, stream)

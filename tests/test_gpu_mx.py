@@ -236,7 +236,8 @@ def test_large_products(m, n, k):
 
 # tiles of 128 x 128 with many stages; few tiles down a long k, whose stages are divided: a short last part, an empty one
 # (17 stages), equal ones, a last stage of one block
-@pytest.mark.parametrize("m, n, k", [(2100, 2200, 1500), (65, 61, 3873), (64, 1000, 4100), (130, 300, 8192), (33, 70, 12289), (1000, 1, 4097)])
+@pytest.mark.parametrize("m, n, k", [(2100, 2200, 1500), (65, 61, 3873), (64, 1000, 4100), (130, 300, 8192), (33, 70, 12289), (1000, 1, 4097),
+                                     (3, 5000, 4000), (1, 16400, 3900), (16, 8200, 4128), (30, 600, 1500)])
 @pytest.mark.parametrize("res_dtype", [np.float16, np.float32])
 def test_products_down_a_long_k(m, n, k, res_dtype):
     mx = _mx()
