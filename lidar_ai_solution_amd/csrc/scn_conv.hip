@@ -111,7 +111,15 @@ bool ConvWeights::init_mx(const uint16_t* w_fp16, const uint16_t* bias_fp16) {
       const int k = g / chunks, b = g % chunks, nv = std::min(32, cin - 32 * b);
       for (int i = 0; i < nv; ++i) v[i] = half_bits_to_float(w_fp16[((size_t)co * kvol + k) * cin + 32 * b + i]);
       const size_t f = ((size_t)g * tiles + co / 32) * 32 + co % 32;
-      sc[(((size_t)g * groups + co / 128) * 32 + co % 32) * 4 + co / 32 % 4] = mx_quantize_block(v, nv, &frag[f * 16]);
+      const uint8_t scale = mx_quantize_block(v, nv, &frag[f * 16]);
+      // The kernels multiply what a row lacks (a neighbour at an offset that other rows of its tile have) as zeros, and zero
+      // times a block that is not finite is a NaN in a row that never meets these weights.
+      if (scale == 255) {
+        set_error("mxfp4 convolution: weights must be finite (output channel %d, kernel offset %d, input channels %d to %d)", co, k,
+                  32 * b, 32 * b + nv - 1);
+        return false;
+      }
+      sc[(((size_t)g * groups + co / 128) * 32 + co % 32) * 4 + co / 32 % 4] = scale;
     }
   if (!zrow.alloc(1536) || !wfrag.alloc(frag.size()) || !wscale.alloc(sc.size()) || !bias.alloc(bs.size() * 4)) return false;
   if (hipMemset(zrow.p, 0, 512) != hipSuccess || hipMemset(zrow.as<char>() + 512, 0xFF, 1024) != hipSuccess ||
