@@ -289,15 +289,18 @@ __device__ __forceinline__ v16f mx_mma32(const uint4& a, int sa, const uint4& b,
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(a), mx_operand(b), c, 4, 4, 0, sa, 0, sb);
 }
 
+// ReLU of a product: a NaN (of a block that is not finite) stays one.
+__device__ __forceinline__ float product_relu(float y) { return y < 0.f ? 0.f : y; }
+
 // Bias, ReLU, residual and store of one element.
 __device__ __forceinline__ void product_store(const ProductArgs& p, uint32_t i, uint32_t j, float y) {
   if (p.bias) y += p.bias_fp32 ? ((const float*)p.bias)[j] : (float)((const _Float16*)p.bias)[j];
-  if (p.relu) y = y > 0.f ? y : 0.f;
+  if (p.relu) y = product_relu(y);
   if (p.res) {
     const size_t at = (size_t)i * p.res_ld + j;
     y += p.res_fp32 ? ((const float*)p.res)[at] : (float)((const _Float16*)p.res)[at];
   }
-  if (p.relu2) y = y > 0.f ? y : 0.f;
+  if (p.relu2) y = product_relu(y);
   const size_t at = (size_t)i * p.out_ld + j;
   if (p.out_fp32) ((float*)p.out)[at] = y;
   else ((_Float16*)p.out)[at] = (_Float16)y;
@@ -446,7 +449,7 @@ __device__ __forceinline__ void product_store8(const ProductArgs& p, uint32_t i,
   }
   if (p.relu) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) y[q] = y[q] > 0.f ? y[q] : 0.f;
+    for (int q = 0; q < 8; ++q) y[q] = product_relu(y[q]);
   }
   if (p.res) {
     if (p.res_fp32) {
@@ -463,7 +466,7 @@ __device__ __forceinline__ void product_store8(const ProductArgs& p, uint32_t i,
   }
   if (p.relu2) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) y[q] = y[q] > 0.f ? y[q] : 0.f;
+    for (int q = 0; q < 8; ++q) y[q] = product_relu(y[q]);
   }
   const size_t at = (size_t)i * p.out_ld + j;
   if (p.out_fp32) {

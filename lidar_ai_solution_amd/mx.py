@@ -228,7 +228,7 @@ def product(a, b: MxRows, bias: Optional[torch.Tensor] = None, relu: bool = Fals
             relu_after_add: bool = False, out_dtype: torch.dtype = torch.float16, num: Optional[torch.Tensor] = None,
             out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """relu2(relu(a b^T + bias) + residual): a is MxRows, or fp16 / fp32 rows that are quantised on the way; b the rows of a
-    weight matrix.  workspace: uint8 scratch for the quantised rows (a new one is allocated when it is needed and not
+    weight matrix.  A NaN stays one through both ReLUs (quantize_rows and the convolutions make it 0).  workspace: uint8 scratch for the quantised rows (a new one is allocated when it is needed and not
     given); calls that may overlap need one each."""
     L = _lib()
     n, index = b.num_rows, b.index

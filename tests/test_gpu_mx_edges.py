@@ -35,3 +35,28 @@ def test_convolution_with_the_largest_weights(cin):
     got = mx.Conv(w).forward(mx.quantize_rows(torch.from_numpy(x).to(DEV)), rb, n_out).double().cpu().numpy()
     R.within(got, y, R.tolerance(y, mag, 27 * cin, 2.0 ** -11))
     assert np.isfinite(y).all() and not np.isnan(got).any()
+
+
+# one row, the few-row kernel, the product's own quantisation, tiles of every size, k in parts
+@pytest.mark.parametrize("m, n, k", [(1, 40, 100), (4, 40, 100), (40, 70, 100), (200, 130, 300), (300, 64, 64), (2050, 2061, 600), (4111, 2300, 300),
+                                     (70, 70, 4000)])
+@pytest.mark.parametrize("x", ["mx", "fp16"])
+@pytest.mark.parametrize("out_dtype", [torch.float16, torch.float32])
+def test_product_relu_keeps_nan(m, n, k, x, out_dtype):
+    mx = _mx()
+    rng = np.random.default_rng(m + n)
+    wh, ah = rng.standard_normal((n, k)).astype(np.float16), rng.standard_normal((m, k)).astype(np.float16)
+    wh[5, k - 1], wh[n - 1, 0] = np.inf, np.nan
+    if m > 1:
+        ah[1, k // 2] = -np.inf
+    w, a = mx.quantize_rows(torch.from_numpy(wh).to(DEV)), torch.from_numpy(ah).to(DEV)
+    a = mx.quantize_rows(a) if x == "mx" else a
+    res = torch.full((m, n), -1.0, dtype=torch.float16, device=DEV)
+    want = np.zeros((m, n), bool)
+    want[:, [5, n - 1]] = True
+    want[1:2] = True
+    for kw in (dict(relu=True), dict(relu_after_add=True), dict(relu=True, residual=res, relu_after_add=True), dict(relu=True, residual=res)):
+        got = mx.product(a, w, out_dtype=out_dtype, **kw).double().cpu().numpy()
+        assert np.array_equal(np.isnan(got), want), kw
+        floor = -1.0 if "residual" in kw and "relu_after_add" not in kw else 0.0
+        assert (got[~want] >= floor).all() and (got[~want] == floor).any(), kw
