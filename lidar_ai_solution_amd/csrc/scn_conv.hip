@@ -157,9 +157,21 @@ int conv_forward(const ConvWeights& w, const int32_t* nbr, uint32_t nbr_ld, cons
   const uint32_t mx_bytes = mx_row_bytes((uint32_t)w.cout);
   if (mx_only) {
     SCN_REQUIRE(conv_stores_mx(w), SCN_ERR_UNSUPPORTED, "conv: microscaled output needs an mxfp4 layer of at most 128 input channels");
-    SCN_REQUIRE(io.out_dev != io.x_dev, SCN_ERR_INVALID, "conv: the output rows must not be the input rows");
     SCN_REQUIRE(io.out_ld >= mx_bytes && io.out_ld % 16 == 0 && ((uintptr_t)io.out_dev & 15) == 0, SCN_ERR_INVALID,
                 "conv: microscaled output rows of %d channels need %u bytes, 16-byte aligned (stride %u)", w.cout, mx_bytes, io.out_ld);
+  }
+  if (w.precision == SCN_PRECISION_MXFP4) {
+    // Rows are gathered while others are stored.  How many rows the arrays have is not known here (the bound may be more than
+    // the count on the device): the first ones are looked at.
+    const auto first = [&](const void* at, int dtype) {
+      return MxSpan{at, 1, dtype == SCN_DTYPE_MXFP4 ? mx_bytes : (uint64_t)w.mtiles * 16 * (dtype == SCN_DTYPE_INT8 ? 1 : 2), 0};
+    };
+    const MxSpan x{io.x_dev, 1, w.cin_pad, 0}, out = first(io.out_dev, io.out_dtype), res = first(io.res_dev, io.res_dtype),
+        acc{io.acc_dev, 1, (uint64_t)w.cout * 4, 0};
+    SCN_REQUIRE(!mx_overlap(out, x) && !mx_overlap(acc, x), SCN_ERR_INVALID, "conv: the output rows must not overlap the input rows");
+    SCN_REQUIRE(!mx_overlap(out, res) || (io.res_dev == io.out_dev && io.res_dtype == io.out_dtype && (io.res_ld == io.out_ld || n_bound == 1)),
+                SCN_ERR_INVALID, "conv: the output must be the residual (of its type and stride) or not overlap it");
+    SCN_REQUIRE(!mx_overlap(acc, out) && !mx_overlap(acc, res), SCN_ERR_INVALID, "conv: the sums must not overlap the output or the residual");
   }
   SCN_REQUIRE(mx_only || io.out_ld >= (uint32_t)w.mtiles * 16, SCN_ERR_INVALID, "conv: output row stride %u < %d", io.out_ld,
               w.mtiles * 16);

@@ -206,6 +206,10 @@ int mx_quantize_rows(const void* in, int in_dtype, uint32_t c, uint32_t in_ld, f
   SCN_REQUIRE(in && ((uintptr_t)in & (esz - 1)) == 0 && in_ld >= c, SCN_ERR_INVALID,
               "mx_quantize_rows: null or misaligned rows, or row stride %u < %u channels", in_ld, c);
   SCN_REQUIRE(in_dtype != SCN_DTYPE_INT8 || in_range > 0.f, SCN_ERR_INVALID, "mx_quantize_rows: int8 rows need in_range > 0");
+  const MxSpan rows{in, n, (uint64_t)c * esz, (uint64_t)in_ld * esz}, cs{codes, n, mx_blocks(c) * kMxBlockBytes, codes_ld},
+      ss{scales, n, mx_scale_bytes(c), scales_ld};
+  SCN_REQUIRE(!mx_overlap(rows, cs) && !mx_overlap(rows, ss) && !mx_overlap(cs, ss), SCN_ERR_INVALID,
+              "mx_quantize_rows: the rows, the codes and the scales must not overlap");
   const FastDiv fd(mx_blocks(c));
   const MxGrid g(n, fd.d, 2 * esz);
 #define SCN_MX_QUANTIZE(DT, ONE)                                                                                          \
@@ -236,6 +240,10 @@ int mx_dequantize_rows(const uint8_t* codes, uint32_t codes_ld, const uint8_t* s
   const uint32_t esz = out_dtype == SCN_DTYPE_FP32 ? 4 : 2;
   SCN_REQUIRE(out && ((uintptr_t)out & (esz - 1)) == 0 && out_ld >= c, SCN_ERR_INVALID,
               "mx_dequantize_rows: null or misaligned output, or row stride %u < %u channels", out_ld, c);
+  const MxSpan rows{out, n, (uint64_t)c * esz, (uint64_t)out_ld * esz};
+  SCN_REQUIRE(!mx_overlap(rows, {codes, n, mx_blocks(c) * kMxBlockBytes, codes_ld}) &&
+                  !mx_overlap(rows, {scales, n, mx_scale_bytes(c), scales_ld}),
+              SCN_ERR_INVALID, "mx_dequantize_rows: the output must not overlap the codes or the scales");
   const FastDiv fd(mx_blocks(c));
   const MxGrid g(n, fd.d, 2 * esz);
   if (out_dtype == SCN_DTYPE_FP16)
@@ -766,8 +774,35 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM, KS>), 2) void k_mx
   }
 }
 
+// What comes in front of a product's launch, once its kernel has taken the sizes: no operand lies where the call writes, and rows
+// that go through the workspace (p.a is that then) are quantised into it.
+static int product_start(const ProductArgs& p, const scn_mx_product_io& io, hipStream_t stream) {
+  const auto size = [](int dtype) -> uint64_t { return dtype == SCN_DTYPE_FP32 ? 4 : 2; };
+  const uint64_t codes = (uint64_t)p.kb * kMxBlockBytes, scales = mx_scale_bytes(p.k);
+  const bool mx = io.a_dtype == SCN_DTYPE_MXFP4, quantise = p.a != io.a_dev;
+  const MxSpan out{io.out_dev, io.m, io.n * size(io.out_dtype), io.out_ld * size(io.out_dtype)},
+      ws{quantise ? p.a : nullptr, 1, (uint64_t)io.m * p.a_ld, 0},
+      res{io.res_dev, io.m, io.n * size(io.res_dtype), io.res_ld * size(io.res_dtype)};
+  const MxSpan read[] = {mx ? MxSpan{io.a_dev, io.m, codes, io.a_ld} : MxSpan{io.a_dev, io.m, io.k * size(io.a_dtype), io.a_ld * size(io.a_dtype)},
+                         {mx ? io.a_scales_dev : nullptr, io.m, scales, io.a_scales_ld},
+                         {io.b_codes_dev, io.n, codes, io.b_codes_ld},
+                         {io.b_scales_dev, io.n, scales, io.b_scales_ld},
+                         {io.bias_dev, 1, io.n * size(io.bias_dtype), 0},
+                         {io.m_dev, 1, 4, 0}};
+  for (const MxSpan& r : read)
+    SCN_REQUIRE(!mx_overlap(out, r) && !mx_overlap(ws, r), SCN_ERR_INVALID,
+                "mx_product: the output and the workspace must not overlap the rows, the weights, the bias or the count");
+  SCN_REQUIRE(io.res_dev == io.out_dev || !mx_overlap(out, res), SCN_ERR_INVALID,
+              "mx_product: the output must be the residual or not overlap it");
+  SCN_REQUIRE(!mx_overlap(ws, out) && !mx_overlap(ws, res), SCN_ERR_INVALID,
+              "mx_product: the workspace must not overlap the output or the residual");
+  if (!quantise) return SCN_OK;
+  return mx_quantize_rows(io.a_dev, io.a_dtype, io.k, io.a_ld, 0.f, 0, static_cast<uint8_t*>(io.workspace_dev), p.a_ld,
+                          const_cast<uint8_t*>(p.as), p.as_ld, io.m, io.m_dev, stream);
+}
+
 template <int BN, int BM, int TN, int TM, int KS>
-static int launch_product(const ProductArgs& p, hipStream_t stream) {
+static int launch_product(const ProductArgs& p, const scn_mx_product_io& io, hipStream_t stream) {
   using T = ProductTile<BN, BM, TN, TM, KS>;
   const uint64_t tn = ((uint64_t)p.n + BN - 1) / BN, tm = ((uint64_t)p.m + BM - 1) / BM;
   SCN_REQUIRE((uint64_t)std::max(std::max(p.a_ld, p.b_ld), std::max(p.as_ld, p.bs_ld)) * 256 < (1ull << 32), SCN_ERR_UNSUPPORTED,
@@ -775,6 +810,7 @@ static int launch_product(const ProductArgs& p, hipStream_t stream) {
   constexpr uint64_t threads = 64 * T::WAVES * KS;   // (a launch has fewer than 2^32 threads)
   SCN_REQUIRE((tn * tm + 7) / 8 * 8 * threads < (1ull << 32), SCN_ERR_UNSUPPORTED, "mx_product: %u x %u outputs are too many for one call",
               p.m, p.n);
+  if (int rc = product_start(p, io, stream)) return rc;
   const uint32_t stages = (p.kb + 7) / 8;
   hipLaunchKernelGGL((k_mx_product_lds<BN, BM, TN, TM, KS>), dim3((unsigned)((tn * tm + 7) / 8 * 8)), dim3((unsigned)threads),
                      KS * T::lds(std::min(T::share(stages), stages)), stream, p, (uint32_t)tn, (uint32_t)tm);
@@ -939,8 +975,9 @@ static void launch_fused(const ProductArgs& p, hipStream_t stream) {
   else launch(k_mx_product_fused<AT, WN, 8>, FusedTile<AT, WN, 8>::BM, FusedTile<AT, WN, 8>::NW);
 }
 template <int AT>
-static int launch_fused(const ProductArgs& p, hipStream_t stream) {
+static int launch_fused(const ProductArgs& p, const scn_mx_product_io& io, hipStream_t stream) {
   SCN_REQUIRE((uint64_t)p.b_ld * 256 < (1ull << 32), SCN_ERR_UNSUPPORTED, "mx_product: rows more than 16 MB apart");
+  if (int rc = product_start(p, io, stream)) return rc;
   if (p.n <= 64) launch_fused<AT, 1>(p, stream);
   else if (p.n <= 128) launch_fused<AT, 2>(p, stream);
   else launch_fused<AT, 4>(p, stream);
@@ -964,9 +1001,10 @@ static size_t product_workspace(uint32_t m, uint32_t n, uint32_t k) {
 
 // U = runs a wave requests at once: what it has to do in all, up to 8 (4 for two row tiles).
 template <int AT, int MT>
-static int launch_few(const ProductArgs& p, hipStream_t stream) {
+static int launch_few(const ProductArgs& p, const scn_mx_product_io& io, hipStream_t stream) {
   const uint32_t runs = (p.kb + 3) / 4, waves = std::min(8u, runs), per = ceil_div(runs, waves);
   SCN_REQUIRE(p.n < (1u << 27), SCN_ERR_UNSUPPORTED, "mx_product: %u x %u outputs are too many for one call", p.m, p.n);
+  if (int rc = product_start(p, io, stream)) return rc;
   const dim3 grid(ceil_div(p.n, 16)), block(64 * waves);
   if (per == 1) hipLaunchKernelGGL((k_mx_product_few<AT, MT, 1>), grid, block, 0, stream, p);
   else if (per == 2) hipLaunchKernelGGL((k_mx_product_few<AT, MT, 2>), grid, block, 0, stream, p);
@@ -991,7 +1029,6 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
   auto aligned = [](const void* p, int dtype) { return ((uintptr_t)p & (dtype == SCN_DTYPE_FP32 ? 3 : 1)) == 0; };
   SCN_REQUIRE(io.out_dev && aligned(io.out_dev, io.out_dtype) && io.out_ld >= io.n, SCN_ERR_INVALID,
               "mx_product: null or misaligned output, or row stride %u < %u", io.out_ld, io.n);
-  SCN_REQUIRE(io.out_dev != io.a_dev, SCN_ERR_INVALID, "mx_product: the output must not be the rows");
   SCN_REQUIRE(aligned(io.bias_dev, io.bias_dtype), SCN_ERR_INVALID, "mx_product: misaligned bias");
   SCN_REQUIRE(!io.res_dev || (aligned(io.res_dev, io.res_dtype) && io.res_ld >= io.n), SCN_ERR_INVALID,
               "mx_product: misaligned residual, or row stride %u < %u", io.res_ld, io.n);
@@ -1034,10 +1071,7 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
       uint8_t* ws = (uint8_t*)io.workspace_dev;
       p.a = ws;
       p.a_ld = p.as_ld = mx_row_bytes(io.k);
-      p.as = ws + (size_t)kb * kMxBlockBytes;
-      if (int rc = mx_quantize_rows(io.a_dev, at, io.k, io.a_ld, 0.f, 0, ws, p.a_ld, const_cast<uint8_t*>(p.as), p.as_ld, io.m,
-                                    io.m_dev, stream))
-        return rc;
+      p.as = ws + (size_t)kb * kMxBlockBytes;   // (product_start quantises the rows into it)
       at = SCN_DTYPE_MXFP4;
     }
   }
@@ -1049,13 +1083,13 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
   const bool few = io.m <= 16 && !(kb > 120 && tiles(64) >= (io.m > 2 ? 72u : 256u));
   int rc;
   if (at != SCN_DTYPE_MXFP4 && !product_direct(io.m, io.k))
-    rc = at == SCN_DTYPE_FP16 ? launch_fused<SCN_DTYPE_FP16>(p, stream) : launch_fused<SCN_DTYPE_FP32>(p, stream);
-  else if (at == SCN_DTYPE_FP16) rc = launch_few<SCN_DTYPE_FP16, 1>(p, stream);
-  else if (at == SCN_DTYPE_FP32) rc = launch_few<SCN_DTYPE_FP32, 1>(p, stream);
-  else if (few) rc = launch_few<SCN_DTYPE_MXFP4, 1>(p, stream);
+    rc = at == SCN_DTYPE_FP16 ? launch_fused<SCN_DTYPE_FP16>(p, io, stream) : launch_fused<SCN_DTYPE_FP32>(p, io, stream);
+  else if (at == SCN_DTYPE_FP16) rc = launch_few<SCN_DTYPE_FP16, 1>(p, io, stream);
+  else if (at == SCN_DTYPE_FP32) rc = launch_few<SCN_DTYPE_FP32, 1>(p, io, stream);
+  else if (few) rc = launch_few<SCN_DTYPE_MXFP4, 1>(p, io, stream);
   // two row tiles of 16 while the tiled kernel below does not divide k: 32 rows, 1024 x 1024 weights 3.5 against 4.0 us, 8192 x 2048
   // 7.4 against 7.1
-  else if (io.m > 16 && io.m <= 32 && kb >= 32 && kb < 64 && io.n <= 4096) rc = launch_few<SCN_DTYPE_MXFP4, 2>(p, stream);
+  else if (io.m > 16 && io.m <= 32 && kb >= 32 && kb < 64 && io.n <= 4096) rc = launch_few<SCN_DTYPE_MXFP4, 2>(p, io, stream);
   else {
     // The largest tile of which there are enough for the GPU's 256 CUs, when k is long enough for its reuse to count.  us for
     // 64 | 128 | 256 rows and channels a tile:
@@ -1066,10 +1100,10 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
     // The smallest tile with k in 4 parts, when there is a CU for every tile and 16 stages: whole | in 4 parts
     //   4096 x 64 x 8192 13.6 | 10.4, 16384 x 64 x 4096 (256 tiles) 12.8 | 10.0; x 2048 6.4 | 6.5; 24576 x 64 x 4096 14 | 17.
     const bool wide = kb > 16 || (io.res_dev && (uint64_t)io.m * io.n >= (16u << 20));
-    rc = tiles(256) >= 144 && io.n > 128 && kb > 8 ? launch_product<256, 256, 4, 2, 1>(p, stream)
-         : tiles(128) >= 256 && io.n > 64 && wide  ? launch_product<128, 128, 2, 2, 1>(p, stream)
-         : tiles(64) <= 256 && kb > 120            ? launch_product<64, 64, 1, 1, 4>(p, stream)
-                                                   : launch_product<64, 64, 1, 1, 1>(p, stream);
+    rc = tiles(256) >= 144 && io.n > 128 && kb > 8 ? launch_product<256, 256, 4, 2, 1>(p, io, stream)
+         : tiles(128) >= 256 && io.n > 64 && wide  ? launch_product<128, 128, 2, 2, 1>(p, io, stream)
+         : tiles(64) <= 256 && kb > 120            ? launch_product<64, 64, 1, 1, 4>(p, io, stream)
+                                                   : launch_product<64, 64, 1, 1, 1>(p, io, stream);
   }
   if (rc) return rc;
   SCN_HIP(hipGetLastError());

@@ -1,6 +1,7 @@
 // Microscaled 4-bit rows (MXFP4): layout, host-side block quantiser and the launchers of scn_mx.hip.
 #pragma once
 
+#include <cstdint>
 #include <cstring>
 
 #include "scn_common.hpp"
@@ -42,6 +43,23 @@ inline uint8_t mx_quantize_block(const float* v, int n, uint8_t codes[16]) {
     codes[i / 2] |= (uint8_t)((code | (sb >> 31 ? 8 : 0)) << (4 * (i & 1)));
   }
   return (uint8_t)e;
+}
+
+// Memory that a call reads or writes: `rows` runs of `width` bytes, `ld` bytes apart.
+struct MxSpan {
+  const void* at;
+  uint64_t rows, width, ld;
+};
+// Whether two of them share a byte.  Rows of the same stride may lie side by side in one array (codes and scales, columns of a
+// wider buffer); of two strides whose ranges meet the answer is yes.
+inline bool mx_overlap(const MxSpan& a, const MxSpan& b) {
+  if (!a.at || !b.at || !a.rows || !b.rows || !a.width || !b.width) return false;
+  const unsigned __int128 pa = (uintptr_t)a.at, pb = (uintptr_t)b.at;   // (no product of 32-bit numbers wraps)
+  if (pa + (a.rows - 1) * a.ld + a.width <= pb || pb + (b.rows - 1) * b.ld + b.width <= pa) return false;
+  const uint64_t ld = a.rows > 1 ? a.ld : b.ld;   // (a single row has no stride of its own)
+  if ((a.rows > 1 && b.rows > 1 && a.ld != b.ld) || (a.rows == 1 && b.rows == 1) || ld == 0) return true;
+  const uint64_t d = (uint64_t)(pb >= pa ? (pb - pa) % ld : (ld - (pa - pb) % ld) % ld);   // where b's rows start behind a's
+  return d < a.width || d + b.width > ld;
 }
 
 int mx_quantize_rows(const void* in, int in_dtype, uint32_t c, uint32_t in_ld, float in_range, int relu, uint8_t* codes,

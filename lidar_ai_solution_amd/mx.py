@@ -168,6 +168,19 @@ def _same_device(index: int, *others) -> None:
             raise ValueError(f"tensors on different devices (rows on cuda:{index})")
 
 
+def _overlap(a, b) -> bool:
+    """Whether two runs of rows (address, rows, bytes of a row, stride in bytes) share a byte; rows of one stride may lie side
+    by side.  (The C library checks its row operators like this; of a convolution it knows only bounds of the row counts.)"""
+    (pa, na, wa, la), (pb, nb, wb, lb) = a, b
+    if pa + (na - 1) * la + wa <= pb or pb + (nb - 1) * lb + wb <= pa or not (na and nb):
+        return False
+    if na > 1 and nb > 1 and la != lb or na == nb == 1:
+        return True
+    ld = la if na > 1 else lb
+    d = (pb - pa) % ld
+    return d < wa or d + wb > ld
+
+
 def quantize_rows(x: torch.Tensor, relu: bool = False, dynamic_range: float = 0.0, num: Optional[torch.Tensor] = None,
                   out: Optional[MxRows] = None, stream=None) -> MxRows:
     """x: fp16, fp32 or int8 (value = q * dynamic_range / 127) rows [n, c]; num: device-side row count (rows beyond it are
@@ -389,6 +402,10 @@ class Conv:
             if out.shape[0] < max_rows or out.shape[1] < wide:
                 raise ValueError(f"out must hold {max_rows} rows of {wide} channels")
             _same_device(x.index, out)
+        n_out = rulebook.rows_out
+        rows_out = (out.codes_ptr, n_out, row_bytes(self.cout), out_ld) if to_mx else (out.data_ptr(), n_out, 2 * wide, 2 * out_ld)
+        if _overlap((x.codes_ptr, rulebook.rows_in, row_bytes(self.cin), x.codes_ld), rows_out):
+            raise RuntimeError("out must not overlap the input rows")
         io = capi.ConvIO()
         io.x_dev, io.x_ld = x.codes_ptr, x.codes_ld
         io.relu, io.out_ld = int(bool(relu)), out_ld
@@ -398,6 +415,9 @@ class Conv:
             if residual.shape[0] < max_rows or residual.shape[1] < wide:
                 raise ValueError(f"residual must hold {max_rows} rows of {wide} channels")
             _same_device(x.index, residual)
+            res = (residual.data_ptr(), n_out, 2 * wide, 2 * io.res_ld)
+            if _overlap(rows_out, res) and (to_mx or res[0] != rows_out[0] or n_out > 1 and res[3] != rows_out[3]):
+                raise RuntimeError("out must be the residual, of the same stride, or not overlap it")
             io.res_dev, io.res_dtype, io.mid_dtype = residual.data_ptr(), capi.DTYPE_FP16, capi.DTYPE_FP16
             io.relu_after_add = int(bool(relu_after_add))
         capi.check(_lib().scn_conv_forward(self._h, rulebook._h, C.byref(io), _stream(x.index)))

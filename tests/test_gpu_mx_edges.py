@@ -60,3 +60,83 @@ def test_product_relu_keeps_nan(m, n, k, x, out_dtype):
         assert np.array_equal(np.isnan(got), want), kw
         floor = -1.0 if "residual" in kw and "relu_after_add" not in kw else 0.0
         assert (got[~want] >= floor).all() and (got[~want] == floor).any(), kw
+
+
+def test_arrays_side_by_side_in_one_buffer():
+    """Columns of one buffer: rows, their codes and scales, the output; nothing overlaps, so nothing is refused."""
+    mx = _mx()
+    rng = np.random.default_rng(1)
+    n = 70
+    buf = torch.zeros((n, 512), dtype=torch.uint8, device=DEV)
+    x = buf[:, :192].view(torch.float16)                                  # 96 channels
+    x.copy_(torch.from_numpy(rows(rng, n, 96)))
+    q = mx.quantize_rows(x, out=mx.MxRows(buf[:, 192:240], buf[:, 240:244], 96))
+    xv = R.fake(x.cpu().numpy())
+    wh = rows(rng, 33, 96)
+    w, wv = mx.quantize_rows(torch.from_numpy(wh).to(DEV)), R.fake(wh)
+    y, mag = R.product(xv, wv)
+    for a in (q, x):
+        out = mx.product(a, w, out=buf[:, 256:322].view(torch.float16))
+        R.within(out.double().cpu().numpy(), y, R.tolerance(y, mag, 96, 2.0 ** -11))
+    back = mx.dequantize_rows(q, out=buf[:, 320:512].view(torch.float16))
+    assert np.array_equal(back.cpu().numpy(), xv.astype(np.float16))
+
+
+def test_convolution_refuses_overlaps():
+    mx = _mx()
+    rng = np.random.default_rng(2)
+    rb, table, n_out, conv, wv, b = conv_case(rng, 200, (9, 24, 21), 64, 64, (3, 3, 3), (1, 1, 1), (1, 1, 1), True)
+    x = rows(rng, 200, 64)
+    buf = torch.zeros((400, 384), dtype=torch.uint8, device=DEV)
+    q = mx.quantize_rows(torch.from_numpy(x).to(DEV), out=mx.MxRows(buf[:200, :32], buf[:200, 32:36], 64))
+
+    def half(first_row, column):
+        return buf[first_row:first_row + 200, column:column + 128].view(torch.float16)
+
+    def mx_out(first_row, column):
+        return mx.MxRows(buf[first_row:first_row + 200, column:column + 32], buf[first_row:first_row + 200, column + 32:column + 36], 64)
+
+    for out in (half(0, 16), half(199, 0), mx_out(0, 16), mx_out(199, 0), buf.flatten()[:200 * 128].view(200, 128).view(torch.float16)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            conv.forward(q, rb, n_out, out=out)
+    for res in (half(0, 80), half(1, 64), half(199, 64)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            conv.forward(q, rb, n_out, out=half(0, 64), residual=res)
+    with pytest.raises(RuntimeError, match="overlap"):
+        conv.forward(q, rb, n_out, out=mx_out(0, 64), residual=half(0, 64))
+    assert not buf[:, 48:].any() and not buf[200:].any()
+    # beside each other, behind each other, and over the residual
+    y, mag = R.convolution(R.fake(x), wv, b, table)
+    tol = R.tolerance(y, mag, 27 * 64, 2.0 ** -11)
+    for out in (half(0, 48), half(200, 0), half(200, 256)):
+        R.within(conv.forward(q, rb, n_out, out=out).double().cpu().numpy(), y, tol)
+    res = rng.standard_normal((200, 64)).astype(np.float16)
+    half(0, 256).copy_(torch.from_numpy(res))
+    want = y + res
+    tol = tol + R.tolerance(want, 0 * mag, 0, 2.0 ** -11)
+    for out in (half(0, 128), half(0, 256)):
+        R.within(conv.forward(q, rb, n_out, out=out, residual=half(0, 256)).double().cpu().numpy(), want, tol)
+
+
+@pytest.mark.parametrize("m", [3, 60, 300])
+def test_product_refuses_overlaps_from_python(m):
+    mx = _mx()
+    w = mx.quantize_rows(torch.randn(24, 320, device=DEV))
+    buf = torch.zeros((m + 2, 320), dtype=torch.float16, device=DEV)
+    a, res = buf[1:m + 1], torch.zeros((m + 1, 24), dtype=torch.float16, device=DEV)
+    q = mx.MxRows.empty(m, 320, DEV)
+    q._buffer.zero_()
+    for x, out in ((a, buf[:m, :24]), (a, buf[2:, 296:]), (q, q._buffer[:48 * m].view(m, 48).view(torch.float16))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            mx.product(x, w, out=out)
+    with pytest.raises(RuntimeError, match="overlap"):
+        mx.product(a, w, out=res[1:], residual=res[:m])
+    if m > 16:
+        with pytest.raises(RuntimeError, match="overlap"):
+            mx.product(a, w, workspace=buf.view(-1).view(torch.uint8))
+    with pytest.raises(RuntimeError, match="overlap"):
+        mx.quantize_rows(a, out=mx.MxRows(buf[:m].view(torch.uint8)[:, :160], buf[:m].view(torch.uint8)[:, 160:172], 320))
+    narrow = mx.MxRows(q.codes[:, :16], q.scales[:, :4], 32)
+    with pytest.raises(RuntimeError, match="overlap"):
+        mx.dequantize_rows(narrow, out=q._buffer[8:8 + 64 * m].view(m, 64).view(torch.float16))
+    assert not buf.any() and not res.any() and not q._buffer.any()

@@ -18,3 +18,74 @@ def test_convolution_refuses_weights_that_are_not_finite(shape, at, where, bad):
     assert not capi.lib().scn_conv_create(w.ctypes.data_as(C.c_void_p), capi.i5(*shape), None, None, capi.PRECISION_MXFP4)
     text = capi.lib().scn_last_error().decode()
     assert "finite" in text and where in text
+
+
+GOOD = 1 << 20   # an aligned address that no refused call reads
+
+
+def _product_io(**over):
+    """40 x 320 rows times 24 weight rows, every array far from the others: rows at 1 MB, weights at 2, and so on."""
+    io = capi.MxProductIO()
+    base = dict(a_dev=GOOD, a_dtype=capi.DTYPE_MXFP4, a_ld=176, a_scales_dev=GOOD + 160, a_scales_ld=176, b_codes_dev=2 * GOOD, b_codes_ld=176,
+                b_scales_dev=2 * GOOD + 160, b_scales_ld=176, m=40, n=24, k=320, bias_dev=3 * GOOD, bias_dtype=capi.DTYPE_FP32,
+                res_dev=4 * GOOD, res_dtype=capi.DTYPE_FP16, res_ld=30, out_dev=5 * GOOD, out_dtype=capi.DTYPE_FP16, out_ld=30,
+                m_dev=6 * GOOD, workspace_dev=7 * GOOD, workspace_bytes=7040)
+    base.update(over)
+    for key, v in base.items():
+        setattr(io, key, v)
+    return io
+
+
+FP16_ROWS = dict(a_dtype=capi.DTYPE_FP16, a_ld=320)
+OVER = [dict(out_dev=GOOD + 39 * 176 + 158),                              # the last row's last codes
+        dict(out_dev=GOOD - 39 * 60 - 46),                                # the last output row, the first codes
+        dict(out_dev=GOOD + 160 + 10), dict(out_dev=2 * GOOD + 23 * 176), dict(out_dev=2 * GOOD + 23 * 176 + 166),
+        dict(out_dev=3 * GOOD + 94), dict(out_dev=4 * GOOD + 2), dict(out_dev=4 * GOOD + 60), dict(out_dev=4 * GOOD - 60),
+        dict(out_dev=4 * GOOD + 36),                                      # columns that run into the next row's
+        dict(out_dev=6 * GOOD), dict(out_dev=GOOD + 100, out_ld=88),      # (stride of the rows, columns of them)
+        dict(FP16_ROWS, out_dev=GOOD + 2), dict(FP16_ROWS, out_dev=GOOD + 39 * 640 + 638), dict(FP16_ROWS, out_dev=GOOD, m=3),
+        dict(FP16_ROWS, workspace_dev=GOOD + 16), dict(FP16_ROWS, workspace_dev=2 * GOOD - 16), dict(FP16_ROWS, workspace_dev=3 * GOOD + 80),
+        dict(FP16_ROWS, workspace_dev=4 * GOOD + 48), dict(FP16_ROWS, workspace_dev=5 * GOOD - 7024), dict(FP16_ROWS, workspace_dev=6 * GOOD - 16)]
+
+
+@pytest.mark.parametrize("over", OVER)
+def test_product_refuses_overlaps(over):
+    assert capi.lib().scn_mx_product(C.byref(_product_io(**over)), None) == 1
+    assert b"overlap" in capi.lib().scn_last_error()
+
+
+@pytest.mark.parametrize("codes, scales, codes_ld, scales_ld", [(GOOD, 3 * GOOD, 32, 4), (GOOD + 4 * 128 + 112, 3 * GOOD, 32, 4),
+                                                                (3 * GOOD, GOOD + 124, 32, 4), (3 * GOOD, GOOD - 4, 32, 4), (3 * GOOD, 3 * GOOD + 28, 48, 48),
+                                                                (3 * GOOD, 3 * GOOD + 4 * 32, 32, 4), (GOOD + 128, 3 * GOOD, 144, 4)])
+def test_quantize_and_dequantize_refuse_overlaps(codes, scales, codes_ld, scales_ld):
+    """Rows of 64 fp16 channels, 5 of them at 1 MB (in the last case every 144 bytes), over their codes or scales."""
+    ld = 72 if codes_ld == 144 else 64
+    L = capi.lib()
+    if codes_ld == 144:
+        codes -= 16                                                       # beside the channels it would be allowed
+    assert L.scn_mx_quantize_rows(GOOD, capi.DTYPE_FP16, 64, ld, 0.0, 0, codes, codes_ld, scales, scales_ld, 5, None, None) == 1
+    assert b"overlap" in L.scn_last_error()
+    if codes < 3 * GOOD or scales < 3 * GOOD:
+        assert L.scn_mx_dequantize_rows(codes, codes_ld, scales, scales_ld, 64, GOOD, capi.DTYPE_FP16, ld, 5, None, None) == 1
+        assert b"overlap" in L.scn_last_error()
+
+
+def test_overlap_of_runs_of_rows():
+    """Against sets of bytes; the answer for two different strides may only err towards yes."""
+    from lidar_ai_solution_amd.mx import _overlap
+    rng = np.random.default_rng(1)
+
+    def bytes_of(s):
+        return {s[0] + r * s[3] + i for r in range(s[1]) for i in range(s[2])}
+
+    seen = [0, 0]
+    for _ in range(20000):
+        la = int(rng.integers(1, 12))
+        lb = la if rng.random() < 0.7 else int(rng.integers(1, 12))
+        a = (100, int(rng.integers(0, 5)), int(rng.integers(1, la + 1)), la)
+        b = (int(rng.integers(60, 140)), int(rng.integers(0, 5)), int(rng.integers(1, lb + 1)), lb)
+        got, want = _overlap(a, b), bool(bytes_of(a) & bytes_of(b))
+        assert got == want or (got and la != lb and a[1] > 1 and b[1] > 1), (a, b)
+        assert _overlap(b, a) == got, (a, b)
+        seen[want] += 1
+    assert min(seen) > 2000
