@@ -801,12 +801,16 @@ static int product_start(const ProductArgs& p, const scn_mx_product_io& io, hipS
                           const_cast<uint8_t*>(p.as), p.as_ld, io.m, io.m_dev, stream);
 }
 
+// Rows of a tile lie at 32-bit offsets from its first one.
+static bool product_near(const ProductArgs& p) {
+  return (uint64_t)std::max(std::max(p.a_ld, p.b_ld), std::max(p.as_ld, p.bs_ld)) * 256 < (1ull << 32);
+}
+
 template <int BN, int BM, int TN, int TM, int KS>
 static int launch_product(const ProductArgs& p, const scn_mx_product_io& io, hipStream_t stream) {
   using T = ProductTile<BN, BM, TN, TM, KS>;
   const uint64_t tn = ((uint64_t)p.n + BN - 1) / BN, tm = ((uint64_t)p.m + BM - 1) / BM;
-  SCN_REQUIRE((uint64_t)std::max(std::max(p.a_ld, p.b_ld), std::max(p.as_ld, p.bs_ld)) * 256 < (1ull << 32), SCN_ERR_UNSUPPORTED,
-              "mx_product: rows more than 16 MB apart");
+  SCN_REQUIRE(product_near(p), SCN_ERR_UNSUPPORTED, "mx_product: rows more than 16 MB apart");
   constexpr uint64_t threads = 64 * T::WAVES * KS;   // (a launch has fewer than 2^32 threads)
   SCN_REQUIRE((tn * tm + 7) / 8 * 8 * threads < (1ull << 32), SCN_ERR_UNSUPPORTED, "mx_product: %u x %u outputs are too many for one call",
               p.m, p.n);
@@ -1080,7 +1084,8 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
   // channels, not per 16.  us few | tiled: 8192 x 8192 weights 1 row 11.0 | 11.9, 4 rows 13.0 | 12.0, 16 rows 17.1 | 12.2; 5000 x 8192 1
   // row 11.0 | 11.4, 16 rows 17.0 | 12.1; 16384 x 4096 (256 tiles) 1 row 11.1 | 9.7; but 4096 x 16384 (64 tiles) 16 rows 17.1 | 20.1,
   // 8192 x 2048 5.8 | 6.9
-  const bool few = io.m <= 16 && !(kb > 120 && tiles(64) >= (io.m > 2 ? 72u : 256u));
+  // (rows too far apart for the tiled kernel's 32-bit offsets stay here as well)
+  const bool few = io.m <= 16 && !(kb > 120 && tiles(64) >= (io.m > 2 ? 72u : 256u) && product_near(p));
   int rc;
   if (at != SCN_DTYPE_MXFP4 && !product_direct(io.m, io.k))
     rc = at == SCN_DTYPE_FP16 ? launch_fused<SCN_DTYPE_FP16>(p, io, stream) : launch_fused<SCN_DTYPE_FP32>(p, io, stream);

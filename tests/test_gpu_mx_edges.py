@@ -140,3 +140,22 @@ def test_product_refuses_overlaps_from_python(m):
     with pytest.raises(RuntimeError, match="overlap"):
         mx.dequantize_rows(narrow, out=q._buffer[8:8 + 64 * m].view(m, 64).view(torch.float16))
     assert not buf.any() and not res.any() and not q._buffer.any()
+
+
+@pytest.mark.parametrize("m, n, k", [(4, 5000, 3900), (16, 8200, 3900), (1, 12300, 3900), (3, 40, 100)])
+@pytest.mark.parametrize("far", ["codes", "scales"])
+def test_product_of_a_few_rows_far_apart(m, n, k, far):
+    """Up to 16 rows may lie 16 MB apart and more, whichever kernel takes that many of them."""
+    mx = _mx()
+    rng = np.random.default_rng(m)
+    w = mx.quantize_rows(torch.from_numpy(rng.standard_normal((n, k)).astype(np.float16)).to(DEV))
+    a = mx.quantize_rows(torch.from_numpy(rng.standard_normal((m, k)).astype(np.float16)).to(DEV))
+    apart = torch.empty((m, (1 << 24) + 16), dtype=torch.uint8, device=DEV)
+    part = getattr(a, far)
+    apart[:, :part.shape[1]] = part
+    parts = dict(codes=a.codes, scales=a.scales)
+    parts[far] = apart[:, :part.shape[1]]
+    got = mx.product(mx.MxRows(parts["codes"], parts["scales"], k), w, out_dtype=torch.float32)
+    av, wv = (R.values(r.codes.cpu().numpy(), r.scales.cpu().numpy(), k) for r in (a, w))
+    y, mag = R.product(av, wv)
+    R.within(got.double().cpu().numpy(), y, R.tolerance(y, mag, k, 2.0 ** -24))
