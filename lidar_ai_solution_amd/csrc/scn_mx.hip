@@ -783,7 +783,7 @@ static int product_start(const ProductArgs& p, const scn_mx_product_io& io, hipS
   const MxSpan out{io.out_dev, io.m, io.n * size(io.out_dtype), io.out_ld * size(io.out_dtype)},
       ws{quantise ? p.a : nullptr, 1, (uint64_t)io.m * p.a_ld, 0},
       res{io.res_dev, io.m, io.n * size(io.res_dtype), io.res_ld * size(io.res_dtype)};
-  const MxSpan read[] = {mx ? MxSpan{io.a_dev, io.m, codes, io.a_ld} : MxSpan{io.a_dev, io.m, io.k * size(io.a_dtype), io.a_ld * size(io.a_dtype)},
+  const MxSpan read[] = {{io.a_dev, io.m, mx ? codes : io.k * size(io.a_dtype), mx ? io.a_ld : io.a_ld * size(io.a_dtype)},
                          {mx ? io.a_scales_dev : nullptr, io.m, scales, io.a_scales_ld},
                          {io.b_codes_dev, io.n, codes, io.b_codes_ld},
                          {io.b_scales_dev, io.n, scales, io.b_scales_ld},
@@ -1080,12 +1080,17 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
     }
   }
   const auto tiles = [&](uint32_t t) { return (uint64_t)ceil_div(io.n, t) * ceil_div(io.m, t); };
-  // Up to 16 rows, except where the tiles of the kernel that divides k between waves fill the GPU: it reads the rows once per 64
-  // channels, not per 16.  us few | tiled: 8192 x 8192 weights 1 row 11.0 | 11.9, 4 rows 13.0 | 12.0, 16 rows 17.1 | 12.2; 5000 x 8192 1
-  // row 11.0 | 11.4, 16 rows 17.0 | 12.1; 16384 x 4096 (256 tiles) 1 row 11.1 | 9.7; but 4096 x 16384 (64 tiles) 16 rows 17.1 | 20.1,
-  // 8192 x 2048 5.8 | 6.9
-  // (rows too far apart for the tiled kernel's 32-bit offsets stay here as well)
-  const bool few = io.m <= 16 && !(kb > 120 && tiles(64) >= (io.m > 2 ? 72u : 256u) && product_near(p));
+  // Up to 16 rows of up to 120 blocks go to the few-row kernel, longer ones to whichever kernel is faster: the time of the few-row
+  // kernel grows with the weight rows and by 2 to 5 % with every row; the tiled ones take a round of the GPU, or two, for 1 row as
+  // for 16.  Up to 256 tiles of 64 weight rows they divide k, beyond they do not.  us few | tiled for 1, 4, 8 and 16 rows of 4096
+  // channels, weights not in a cache:
+  //   8192 weight rows (128 tiles) 7.8 8.5 9.4 11.0 | 9.7 9.8 10.0 10.4; 12288 9.8 11.0 12.4 14.8 | 10.2 10.4 10.6 10.9;
+  //   16384 (256) 11.8 13.5 15.4 18.6 | 11.2 11.2 11.4 11.7; 16448 13.6 16.1 18.0 21.8 | 16.6 16.6 16.8 17.0;
+  //   24576 16.9 19.0 21.4 26.6 | 17.9 17.9 18.0 18.2; 32768 21.3 24.2 27.4 34.4 | 19.1 19.1 19.3 19.4.
+  // Rows too far apart for the tiled kernels' 32-bit offsets stay with the few-row kernel.
+  const uint64_t t64 = tiles(64);
+  const bool sooner = t64 <= 256 ? io.m <= 8 && t64 <= (io.m > 1 ? 160u : 192u) : t64 + 20 * io.m < 410;
+  const bool few = io.m <= 16 && (kb <= 120 || t64 < 72 || sooner || !product_near(p));
   int rc;
   if (at != SCN_DTYPE_MXFP4 && !product_direct(io.m, io.k))
     rc = at == SCN_DTYPE_FP16 ? launch_fused<SCN_DTYPE_FP16>(p, io, stream) : launch_fused<SCN_DTYPE_FP32>(p, io, stream);
@@ -1105,10 +1110,12 @@ int mx_product(const scn_mx_product_io& io, hipStream_t stream) {
     // The smallest tile with k in 4 parts, when there is a CU for every tile and 16 stages: whole | in 4 parts
     //   4096 x 64 x 8192 13.6 | 10.4, 16384 x 64 x 4096 (256 tiles) 12.8 | 10.0; x 2048 6.4 | 6.5; 24576 x 64 x 4096 14 | 17.
     const bool wide = kb > 16 || (io.res_dev && (uint64_t)io.m * io.n >= (16u << 20));
-    rc = tiles(256) >= 144 && io.n > 128 && kb > 8 ? launch_product<256, 256, 4, 2, 1>(p, io, stream)
-         : tiles(128) >= 256 && io.n > 64 && wide  ? launch_product<128, 128, 2, 2, 1>(p, io, stream)
-         : tiles(64) <= 256 && kb > 120            ? launch_product<64, 64, 1, 1, 4>(p, io, stream)
-                                                   : launch_product<64, 64, 1, 1, 1>(p, io, stream);
+    // Up to 16 rows take no larger tile: 65536 x 4096 weights 31 | 30 | 39, 32768 x 8192 36 | 40 | 43.
+    const bool many = io.m > 16;
+    rc = many && tiles(256) >= 144 && io.n > 128 && kb > 8 ? launch_product<256, 256, 4, 2, 1>(p, io, stream)
+         : many && tiles(128) >= 256 && io.n > 64 && wide  ? launch_product<128, 128, 2, 2, 1>(p, io, stream)
+         : t64 <= 256 && kb > 120                          ? launch_product<64, 64, 1, 1, 4>(p, io, stream)
+                                                           : launch_product<64, 64, 1, 1, 1>(p, io, stream);
   }
   if (rc) return rc;
   SCN_HIP(hipGetLastError());

@@ -159,3 +159,35 @@ def test_product_of_a_few_rows_far_apart(m, n, k, far):
     av, wv = (R.values(r.codes.cpu().numpy(), r.scales.cpu().numpy(), k) for r in (a, w))
     y, mag = R.product(av, wv)
     R.within(got.double().cpu().numpy(), y, R.tolerance(y, mag, k, 2.0 ** -24))
+
+
+@pytest.mark.parametrize("m, n, k", [(1, 16448, 4096), (4, 17000, 3900), (4, 8192, 8192), (8, 10240, 4000), (2, 20000, 3900)])
+def test_few_rows_stay_with_the_kernel_of_few_rows(m, n, k):
+    """... beside as many weight rows as it is the faster one for: its sums, bit for bit, which the tiled kernels add in
+    another order.  (Blocks of very different strength: the sums have to be rounded.)"""
+    mx = _mx()
+    torch.manual_seed(m)
+    strength = torch.exp2(torch.randint(-10, 11, (-(-k // 32),), device=DEV).float()).repeat_interleave(32)[:k]
+    w = mx.quantize_rows(torch.randn(n, k, device=DEV) * strength)
+    a = mx.quantize_rows(torch.randn(m, k, device=DEV) * strength)
+    got = mx.product(a, w, out_dtype=torch.float32)
+    for first in (0, n // 2, n - 640):
+        part = mx.product(a, mx.MxRows(w.codes[first:first + 640], w.scales[first:first + 640], k), out_dtype=torch.float32)
+        assert torch.equal(got[:, first:first + 640], part)
+
+
+# either side of 72, 160 (one row: 192) and 256 tiles of 64 weight rows, of 8 rows, and of the sum of both beyond 256; many weight rows
+@pytest.mark.parametrize("m, n, k", [(1, 4544, 3900), (9, 4545, 3872), (8, 10240, 3900), (8, 10241, 3900), (2, 12300, 4100), (16, 16384, 3880),
+                                     (4, 16385, 3900), (8, 16385, 3900), (16, 17000, 4097), (1, 24900, 3900), (1, 25000, 3900), (1, 37000, 3872),
+                                     (13, 37000, 3872), (1, 12288, 3900), (1, 12289, 3900)])
+def test_few_rows_beside_many_weight_rows(m, n, k):
+    mx = _mx()
+    torch.manual_seed(m + n)
+    wh, ah = torch.randn(n, k, device=DEV).half(), torch.randn(m, k, device=DEV).half()
+    w, a = mx.quantize_rows(wh), mx.quantize_rows(ah)
+    wv, av = (mx.dequantize_rows(r, torch.float32).double() for r in (w, a))     # (exact in fp32)
+    bias = torch.randn(n, device=DEV)
+    y, mag = (av @ wv.T + bias).cpu().numpy(), (av.abs() @ wv.abs().T + bias.abs()).cpu().numpy()
+    for x in (a, ah):
+        got = mx.product(x, w, bias=bias, out_dtype=torch.float32).double().cpu().numpy()
+        R.within(got, y, R.tolerance(y, mag, k, 2.0 ** -24))
