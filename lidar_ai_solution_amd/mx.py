@@ -107,6 +107,8 @@ class MxRows:
         buf = torch.empty(n * size, dtype=torch.uint8, device=device)     # (flat: made in two thirds of the time)
         self._codes = self._scales = None
         self._buffer, self.channels, self.num_rows, self.index = buf, channels, n, buf.get_device()
+        if self.index < 0:
+            raise ValueError(f"rows live on a GPU, not on {buf.device}")
         self.codes_ptr = ptr = buf.data_ptr()
         self.scales_ptr = ptr + 16 * blocks
         self.codes_ld = self.scales_ld = size

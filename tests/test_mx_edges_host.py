@@ -89,3 +89,9 @@ def test_overlap_of_runs_of_rows():
         assert _overlap(b, a) == got, (a, b)
         seen[want] += 1
     assert min(seen) > 2000
+
+
+def test_rows_live_on_a_gpu():
+    from lidar_ai_solution_amd import mx
+    with pytest.raises(ValueError, match="GPU"):
+        mx.MxRows.empty(4, 64, "cpu")
