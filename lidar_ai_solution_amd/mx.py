@@ -317,14 +317,17 @@ class Rulebook:
         self.max_in, self.max_out = int(max_in), int(max_out)
         self.rows_in = self.rows_out = None   # bounds of the last build: rows the convolution may read / write
 
-    def _check(self, indices: torch.Tensor):
+    def _check(self, indices: torch.Tensor, stream):
+        there = getattr(stream, "device_index", self.index)
+        if there != self.index:
+            raise ValueError(f"a stream of cuda:{there} for a rulebook on cuda:{self.index}")
         if indices.dtype != torch.int32 or indices.dim() != 2 or indices.shape[1] != 4 or not indices.is_contiguous() or not indices.is_cuda:
             raise ValueError("indices must be a contiguous int32 device tensor [n, 4]")
         if not indices.get_device() == self.index == _current_device():
             raise ValueError(f"the rulebook lives on cuda:{self.index}: indices and the current device must be that one")
 
     def build_subm(self, indices: torch.Tensor, grid: Sequence[int], kernel_size, dilation=(1, 1, 1), num=None, stream=None):
-        self._check(indices)
+        self._check(indices, stream)
         self._keep = (indices, num)
         capi.check(capi.lib().scn_rulebook_build_subm(
             self._h, indices.data_ptr(), int(indices.shape[0]), _count_ptr(num, indices.get_device()), capi.i3(*grid),
@@ -333,7 +336,7 @@ class Rulebook:
 
     def build_sparse(self, indices: torch.Tensor, grid: Sequence[int], kernel_size, stride, padding, dilation=(1, 1, 1),
                      num=None, stream=None):
-        self._check(indices)
+        self._check(indices, stream)
         self._keep = (indices, num)
         capi.check(capi.lib().scn_rulebook_build_sparse(
             self._h, indices.data_ptr(), int(indices.shape[0]), _count_ptr(num, indices.get_device()), capi.i3(*grid),

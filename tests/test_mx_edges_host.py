@@ -95,3 +95,17 @@ def test_rows_live_on_a_gpu():
     from lidar_ai_solution_amd import mx
     with pytest.raises(ValueError, match="GPU"):
         mx.MxRows.empty(4, 64, "cpu")
+
+
+def test_rulebook_refuses_a_stream_of_another_device():
+    """(The device is checked before anything else, so that a stand-in for a stream does.)"""
+    from types import SimpleNamespace
+
+    from lidar_ai_solution_amd import mx
+    rb = mx.Rulebook.__new__(mx.Rulebook)
+    rb.index = 0
+    there = SimpleNamespace(device_index=1, cuda_stream=0)
+    with pytest.raises(ValueError, match="stream of cuda:1"):
+        rb.build_subm(None, (9, 9, 9), (3, 3, 3), stream=there)
+    with pytest.raises(ValueError, match="stream of cuda:1"):
+        rb.build_sparse(None, (9, 9, 9), (3, 3, 3), (2, 2, 2), (1, 1, 1), stream=there)
