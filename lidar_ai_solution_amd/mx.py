@@ -328,6 +328,7 @@ class Rulebook:
 
     def build_subm(self, indices: torch.Tensor, grid: Sequence[int], kernel_size, dilation=(1, 1, 1), num=None, stream=None):
         self._check(indices, stream)
+        self.rows_in = self.rows_out = None     # (a build that fails leaves no table that may be read)
         self._keep = (indices, num)
         capi.check(capi.lib().scn_rulebook_build_subm(
             self._h, indices.data_ptr(), int(indices.shape[0]), _count_ptr(num, indices.get_device()), capi.i3(*grid),
@@ -337,6 +338,7 @@ class Rulebook:
     def build_sparse(self, indices: torch.Tensor, grid: Sequence[int], kernel_size, stride, padding, dilation=(1, 1, 1),
                      num=None, stream=None):
         self._check(indices, stream)
+        self.rows_in = self.rows_out = None     # (a build that fails leaves no table that may be read)
         self._keep = (indices, num)
         capi.check(capi.lib().scn_rulebook_build_sparse(
             self._h, indices.data_ptr(), int(indices.shape[0]), _count_ptr(num, indices.get_device()), capi.i3(*grid),

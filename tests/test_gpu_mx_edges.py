@@ -191,3 +191,19 @@ def test_few_rows_beside_many_weight_rows(m, n, k):
     for x in (a, ah):
         got = mx.product(x, w, bias=bias, out_dtype=torch.float32).double().cpu().numpy()
         R.within(got, y, R.tolerance(y, mag, k, 2.0 ** -24))
+
+
+def test_rulebook_whose_build_failed_is_not_read():
+    """Neither the old table nor half of a new one."""
+    mx = _mx()
+    rng = np.random.default_rng(6)
+    rb, _, n_out, conv, _, _ = conv_case(rng, 50, (9, 24, 21), 64, 32, (3, 3, 3), (1, 1, 1), (1, 1, 1), True)
+    q = mx.quantize_rows(torch.zeros((50, 64), dtype=torch.float16, device=DEV))
+    conv.forward(q, rb, n_out)
+    idx = torch.zeros((5, 4), dtype=torch.int32, device=DEV)
+    with pytest.raises(RuntimeError):
+        rb.build_sparse(idx, (9, 24, 21), (3, 3, 3), (1, 1, 1), (-1, 0, 0))
+    with pytest.raises(ValueError, match="built"):
+        conv.forward(q, rb, n_out)
+    rb.build_subm(idx, (9, 24, 21), (3, 3, 3))
+    conv.forward(q, rb, n_out)
