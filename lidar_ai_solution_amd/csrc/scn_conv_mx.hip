@@ -99,14 +99,14 @@ struct ConvMxStage {
 };
 
 // 64 x 16 bytes to LDS, lane l's to base + 16 l: in assembly, because the compiler would order its own LDS
-// reads behind every such load in flight.  m0 has no other user in this kernel.
+// reads behind every such load in flight.
 __device__ __forceinline__ void conv_load16_lds(const void* src, uint32_t base) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(base) : "m0", "memory");
 }
 
 // The same of a buffer: bytes [at, at + 16) of it, zeros beyond its size.
 __device__ __forceinline__ void conv_load16_lds(const v4i& buffer, uint32_t at, uint32_t base) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(at), "s"(buffer), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(at), "s"(buffer), "s"(base) : "m0", "memory");
 }
 
 // MODE: the epilogue (see epilogue_values): 2 and 4 are fp16 output without and with an fp16 residual, 0 everything.

@@ -506,13 +506,12 @@ typedef __attribute__((address_space(3))) void* mx_lptr;
 // 64 x 16 (or 64 x 4) bytes from memory to LDS, lane l's to base + 16 l (4 l).  Written in assembly so that the compiler's
 // own LDS reads are not ordered after every load in flight (it would drain them all); the waits are the explicit counts
 // in the kernel.  The address is a wave's base with a 32-bit offset per lane.  The instruction takes its LDS address from m0,
-// which needs one wait state after it is written; nothing else in a kernel that uses these may use m0 (the compiler does for
-// its own loads to LDS, messages and indexed registers, of which there are none).
+// which needs one wait state after it is written.
 __device__ __forceinline__ void mx_load16_lds(const uint8_t* src, uint32_t offset, uint32_t base) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(src), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(src), "s"(base) : "m0", "memory");
 }
 __device__ __forceinline__ void mx_load4_lds(const uint8_t* src, uint32_t offset, uint32_t base) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(src), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(src), "s"(base) : "m0", "memory");
 }
 
 // (the byte of the scale registers is an immediate of the instruction)

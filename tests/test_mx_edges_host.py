@@ -109,3 +109,20 @@ def test_rulebook_refuses_a_stream_of_another_device():
         rb.build_subm(None, (9, 9, 9), (3, 3, 3), stream=there)
     with pytest.raises(ValueError, match="stream of cuda:1"):
         rb.build_sparse(None, (9, 9, 9), (3, 3, 3), (2, 2, 2), (1, 1, 1), stream=there)
+
+
+def test_assembly_that_writes_m0_says_so():
+    """The compiler keeps values of its own in m0 (loads to LDS, indexed registers); a statement that writes it names it."""
+    import glob
+    import os
+    import re
+    src = os.path.join(os.path.dirname(os.path.abspath(capi.__file__)), "csrc")
+    found = 0
+    for path in glob.glob(os.path.join(src, "*.h*")):
+        with open(path) as f:
+            text = f.read()
+        for statement in re.findall(r"\basm\b[^;]*?\((?:[^;\"]|\"[^\"]*\")*\);", text):
+            if re.search(r"\bs_\w+\s+m0\b", statement):
+                found += 1
+                assert re.search(r":[^:]*\"m0\"[^:]*\);$", statement), (path, statement)
+    assert found >= 4
