@@ -995,8 +995,9 @@ static bool product_direct(uint32_t m, uint32_t k) { return m <= 16 && (uint64_t
 // for 256 channels.  us with the two launches | one, fp16 rows: 123646 x 256 x 128 with residual 41.5 | 34.9, 123646 x 64 x 64 14.1 |
 // 8.7, 50000 x 1024 x 64 29.5 | 27.8, 20000 x 1000 x 100 27.6 | 24.6, 50000 x 256 x 256 19.6 | 19.7 (fp32 30.5 | 25.0), 500 x 64 x 256
 // 5.4 | 5.2; but 50000 x 512 x 256 23.6 | 25.7, 5000 x 1024 x 256 8.0 | 9.4.  One launch is 6 us less on the host.
+// (its longest rows take 8 threads each, and a launch has fewer than 2^32)
 static bool product_fused(uint32_t m, uint32_t n, uint32_t k) {
-  return m < (1u << 29) && (k <= 128 ? n <= 1024 : k <= 256 && n <= 256);
+  return m < (1u << 29) - 64 && (k <= 128 ? n <= 1024 : k <= 256 && n <= 256);
 }
 static size_t product_workspace(uint32_t m, uint32_t n, uint32_t k) {
   return product_direct(m, k) || product_fused(m, n, k) ? 0 : (size_t)m * mx_row_bytes(k);

@@ -126,3 +126,11 @@ def test_assembly_that_writes_m0_says_so():
                 found += 1
                 assert re.search(r":[^:]*\"m0\"[^:]*\);$", statement), (path, statement)
     assert found >= 4
+
+
+def test_rows_quantised_in_the_products_launch_fit_it():
+    """64 rows of more than 128 channels are 512 threads: the last row counts below 2^29 would make 2^32."""
+    L = capi.lib()
+    assert L.scn_mx_product_workspace((1 << 29) - 65, 64, 256) == 0
+    for m in ((1 << 29) - 64, (1 << 29) - 1, 1 << 29):
+        assert L.scn_mx_product_workspace(m, 64, 256) == m * L.scn_mx_row_bytes(256)
