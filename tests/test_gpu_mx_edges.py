@@ -207,3 +207,122 @@ def test_rulebook_whose_build_failed_is_not_read():
         conv.forward(q, rb, n_out)
     rb.build_subm(idx, (9, 24, 21), (3, 3, 3))
     conv.forward(q, rb, n_out)
+
+
+# ------------------------------------------------------------------------------------------------- one row, one column
+def signed_rows(rng, n, c, dtype=np.float16):
+    """Rows without a zero channel."""
+    x = (rng.uniform(0.5, 2, (n, c)) * rng.choice([-1, 1], (n, c)) * np.exp(rng.standard_normal((n, 1)))).astype(dtype)
+    assert x.all()
+    return x
+
+
+@pytest.mark.parametrize("m, n, k", [(1, 1, 1), (1, 1, 33), (1, 16, 32), (1, 33, 100), (1, 70, 1000), (1, 500, 8192), (1, 40, 33000), (1, 16400, 3900),
+                                     (1, 12300, 4100), (2, 1, 5000), (16, 1, 70), (17, 1, 3), (300, 1, 64), (300, 1, 300), (40, 1, 1500), (1000, 1, 4097)])
+@pytest.mark.parametrize("x", ["mx", "fp16", "fp32"])
+def test_product_of_one_row_or_one_column(m, n, k, x):
+    mx = _mx()
+    rng = np.random.default_rng(m * 7 + n * 3 + k)
+    wh, h = signed_rows(rng, n, k), signed_rows(rng, m, k, np.float32 if x == "fp32" else np.float16)
+    w, a = mx.quantize_rows(torch.from_numpy(wh).to(DEV)), torch.from_numpy(h).to(DEV)
+    bias, res = rng.standard_normal(n).astype(np.float32), rng.standard_normal((m, n)).astype(np.float16)
+    kw = dict(bias=torch.from_numpy(bias).to(DEV), residual=torch.from_numpy(res).to(DEV))
+    y, mag = R.product(R.fake(h), R.fake(wh), bias, False, res, False)
+    a = mx.quantize_rows(a) if x == "mx" else a
+    for out_dtype, half in ((torch.float16, 2.0 ** -11), (torch.float32, 2.0 ** -24)):
+        got = mx.product(a, w, out_dtype=out_dtype, **kw)
+        R.within(got.double().cpu().numpy(), y, R.tolerance(y, mag, k, half))
+        assert torch.equal(mx.product(a, w, out_dtype=out_dtype, **kw), got)
+
+
+def test_convolution_of_one_row():
+    mx = _mx()
+    rng = np.random.default_rng(5)
+    for cin, cout in ((5, 16), (64, 64), (128, 40), (160, 32)):
+        rb, table, n_out, conv, wv, b = conv_case(rng, 1, (9, 24, 21), cin, cout, (3, 3, 3), (1, 1, 1), (1, 1, 1), True)
+        x = signed_rows(rng, 1, cin)
+        y, mag = R.convolution(R.fake(x), wv, b, table)
+        assert np.abs(y - b).max() > 0.01
+        got = conv.forward(mx.quantize_rows(torch.from_numpy(x).to(DEV)), rb, n_out).double().cpu().numpy()
+        R.within(got, y, R.tolerance(y, mag, 27 * cin, 2.0 ** -11))
+
+
+# ------------------------------------------------------------------------------------------------- sums without a rounding
+def whole(rng, n, k, only_from=0):
+    """Rows of codes under a scale of 1, the channels before `only_from` zero, at least one other that is not: (MxRows, values).
+    Products are quarters up to 36, so that fp32 holds every sum of fewer than 2^24 / 144 = 116,508 of them exactly."""
+    mx = _mx()
+    blocks = -(-k // 32)
+    code = rng.integers(0, 16, (n, 32 * blocks)).astype(np.uint8)
+    code[:, :only_from] = 0
+    code[:, k:] = 0
+    code[:, k - 1] |= 1
+    codes = code[:, 0::2] | (code[:, 1::2] << 4)
+    scales = np.zeros((n, -(-blocks // 4) * 4), np.uint8)
+    scales[:, :blocks] = 127
+    r = mx.MxRows.empty(n, k, DEV)
+    r.codes.copy_(torch.from_numpy(codes))
+    r.scales.copy_(torch.from_numpy(scales))
+    return r, R.values(codes, scales, k)
+
+
+# every kernel and tile, stages and scale spans of every length, k in parts of unequal length
+WHOLE = [(1, 70, 100), (3, 40, 4096), (16, 33, 8190), (20, 100, 1500), (40, 70, 33), (65, 61, 3873), (64, 1000, 4100), (130, 300, 8192), (33, 70, 12289),
+         (1000, 1, 4097), (16, 8200, 4128), (1, 12300, 3900), (16, 17000, 3900), (100, 130, 257), (100, 130, 513), (100, 130, 769), (300, 200, 1111),
+         (2100, 2200, 1500), (2177, 2049, 515), (4100, 4111, 290), (4111, 4099, 2080)]
+
+
+@pytest.mark.parametrize("m, n, k", WHOLE)
+def test_products_add_every_block_once(m, n, k):
+    """Equal to the sums, over all channels and with only the last block, the last few blocks or the last stage not zero."""
+    mx = _mx()
+    rng = np.random.default_rng(m + n + k)
+    last = (k - 1) // 32 * 32
+    for first in sorted({0, last, max(0, last - 96), max(0, last // 256 * 256)}):
+        w, wv = whole(rng, n, k, first)
+        a, av = whole(rng, m, k)
+        got = mx.product(a, w, out_dtype=torch.float32)
+        want = torch.from_numpy(av.astype(np.float32)).to(DEV).double() @ torch.from_numpy(wv.astype(np.float32)).to(DEV).double().T
+        assert want.any() and torch.equal(got.double(), want), first
+
+
+@pytest.mark.parametrize("m, n, k", [(5, 70, 200), (100, 64, 31), (70, 300, 96), (200, 1000, 128), (130, 200, 250), (64, 64, 256), (40, 300, 1111)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_products_that_quantise_add_every_block_once(m, n, k, dtype):
+    """Rows whose channels are values of the format: a 6 in every block makes its scale 1, so quantisation keeps them."""
+    mx = _mx()
+    rng = np.random.default_rng(m + n + k)
+    w, wv = whole(rng, n, k)
+    _, av = whole(rng, m, k)
+    av[:, ::32] = 6
+    got = mx.product(torch.from_numpy(av).to(dtype).to(DEV), w, out_dtype=torch.float32).double().cpu().numpy()
+    assert np.array_equal(got, av @ wv.T)
+
+
+@pytest.mark.parametrize("cin, cout, n, bound", [(16, 16, 500, 500), (32, 64, 500, 40000), (64, 64, 500, 500), (64, 128, 500, 70000), (96, 48, 300, 300),
+                                                 (128, 32, 400, 200000), (160, 96, 200, 200), (256, 128, 90, 90)])
+@pytest.mark.parametrize("ks", [(3, 3, 3), (5, 3, 3), (1, 1, 1)])
+def test_convolutions_add_every_neighbour_once(cin, cout, n, bound, ks):
+    """The sums that the kernel dumps, equal to whole numbers (quarters)."""
+    import ctypes as C
+    mx = _mx()
+    rng = np.random.default_rng(cin + cout)
+    coords = np.stack(np.unravel_index(np.sort(rng.choice(9 * 24 * 21, n, replace=False)), (9, 24, 21)), 1)
+    idx = torch.zeros((bound, 4), dtype=torch.int32, device=DEV)
+    idx[:n, 1:] = torch.from_numpy(coords.astype(np.int32)).to(DEV)
+    kv = int(np.prod(ks))
+    rb = mx.Rulebook(bound, bound, kv)
+    rb.build_subm(idx, (9, 24, 21), ks, num=torch.tensor([n], dtype=torch.int32, device=DEV))
+    _, table = R.neighbours(coords, (9, 24, 21), ks, (1, 1, 1), (1, 1, 1), (1, 1, 1), True)
+    q, xv = whole(rng, n, cin)
+    w = rng.choice(R.LEVELS, (cout, kv, cin)) * rng.choice([-1, 1], (cout, kv, cin))
+    w[:, :, ::32] = 6
+    conv = mx.Conv(w.reshape(cout, *ks, cin).astype(np.float16))
+    acc = torch.full((n, cout), 7.0, device=DEV)
+    out = torch.empty((n, cout), dtype=torch.float16, device=DEV)
+    io = capi.ConvIO()
+    io.x_dev, io.x_ld, io.out_dtype = q.codes_ptr, q.codes_ld, capi.DTYPE_FP16
+    io.out_dev, io.out_ld, io.acc_dev = out.data_ptr(), cout, acc.data_ptr()
+    capi.check(capi.lib().scn_conv_forward(conv._h, rb._h, C.byref(io), torch.cuda.current_stream().cuda_stream))
+    y, _ = R.convolution(xv, w, None, table)
+    assert np.array_equal(acc.double().cpu().numpy(), y)
