@@ -227,7 +227,7 @@ def test_product_of_one_row_or_one_column(m, n, k, x):
     w, a = mx.quantize_rows(torch.from_numpy(wh).to(DEV)), torch.from_numpy(h).to(DEV)
     bias, res = rng.standard_normal(n).astype(np.float32), rng.standard_normal((m, n)).astype(np.float16)
     kw = dict(bias=torch.from_numpy(bias).to(DEV), residual=torch.from_numpy(res).to(DEV))
-    y, mag = R.product(R.fake(h), R.fake(wh), bias, False, res, False)
+    y, mag = R.product(R.fake(h), R.values(w.codes.cpu().numpy(), w.scales.cpu().numpy(), k), bias, False, res, False)
     a = mx.quantize_rows(a) if x == "mx" else a
     for out_dtype, half in ((torch.float16, 2.0 ** -11), (torch.float32, 2.0 ** -24)):
         got = mx.product(a, w, out_dtype=out_dtype, **kw)
