@@ -12,16 +12,20 @@ typedef float v2f __attribute__((ext_vector_type(2)));
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
-// 16 bytes to an address of any alignment, past the L2 (results that no workgroup of this launch reads again).  Ordinary
-// stores make the write-back L2 the bottleneck: dequantising 16,384 x 8,192 to fp16 takes 84 us with them, 47 us with these.
+// 16 bytes to an address of any alignment.  STREAM: past the L2 (results that no workgroup of this launch reads again).  Where a
+// wave writes whole lines, or nearly, ordinary stores make the write-back L2 the bottleneck: us streaming | ordinary, dequantising
+// 16,384 x 8,192 to fp16 52 | 66, to fp32 88 | 123, 50,000 x 1000 to fp16 21.7 | 27.9, 322,224 x 60 to fp16 16.1 | 20.5.
 typedef uint32_t v4u_any __attribute__((ext_vector_type(4), aligned(2)));
-__device__ __forceinline__ void store16_streaming(void* dst, const void* src) {
+template <bool STREAM>
+__device__ __forceinline__ void store16(void* dst, const void* src) {
   v4u_any q;
   __builtin_memcpy(&q, src, 16);
-  __builtin_nontemporal_store(q, reinterpret_cast<v4u_any*>(dst));
+  if (STREAM) __builtin_nontemporal_store(q, reinterpret_cast<v4u_any*>(dst));
+  else *reinterpret_cast<v4u_any*>(dst) = q;
 }
 
-// u / d for u < 2^31 by one high multiplication (d >= 1).
+// u / d for u < 2^31 by one high multiplication (d >= 1): the round-up method of Granlund and Montgomery (Division by Invariant
+// Integers using Multiplication, 1994).
 struct FastDiv {
   uint32_t d, mul, shift;
   explicit FastDiv(uint32_t d_) : d(d_), shift(0) {
@@ -163,7 +167,7 @@ __global__ __launch_bounds__(256) void k_mx_dequantize(const uint8_t* codes, uin
   const uint32_t ch = b * 32 + sub * E;
   OT* dst = out + row * out_ld + ch;
   if (ch + E <= c) {
-    store16_streaming(dst, v);
+    store16<true>(dst, v);
   } else {
 #pragma unroll
     for (int i = 0; i < E; ++i)
@@ -432,7 +436,8 @@ __global__ __launch_bounds__(512) void k_mx_product_few(const ProductArgs p) {
 }
 
 // Bias, ReLU, residual and store of 8 consecutive channels of one row, from LDS (one 16-byte store in fp16, two in fp32;
-// rows of any alignment).  `pre`: the fp16 residual, if there is one.
+// rows of any alignment).  `pre`: the fp16 residual, if there is one.  STREAM: see whole_lines.
+template <bool STREAM>
 __device__ __forceinline__ void product_store8(const ProductArgs& p, uint32_t i, uint32_t j, const float* src, const v4u pre) {
   if (j + 8 > p.n) {
 #pragma unroll 1
@@ -478,13 +483,13 @@ __device__ __forceinline__ void product_store8(const ProductArgs& p, uint32_t i,
   }
   const size_t at = (size_t)i * p.out_ld + j;
   if (p.out_fp32) {
-    store16_streaming((float*)p.out + at, y);
-    store16_streaming((float*)p.out + at + 4, y + 4);
+    store16<STREAM>((float*)p.out + at, y);
+    store16<STREAM>((float*)p.out + at + 4, y + 4);
   } else {
     _Float16 h[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) h[q] = (_Float16)y[q];
-    store16_streaming((_Float16*)p.out + at, h);
+    store16<STREAM>((_Float16*)p.out + at, h);
   }
 }
 
@@ -543,7 +548,7 @@ struct ProductTile {
 template <int BN, int BM, int TN, int TM, int KS>
 constexpr int kProductThreads = 64 * ProductTile<BN, BM, TN, TM, KS>::WAVES * KS;
 
-template <int BN, int BM, int TN, int TM, int KS>
+template <int BN, int BM, int TN, int TM, int KS, bool STREAM>
 __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM, KS>), 2) void k_mx_product_lds(const ProductArgs p, uint32_t tiles_n,
                                                                                               uint32_t tiles_m) {
   using T = ProductTile<BN, BM, TN, TM, KS>;
@@ -768,7 +773,7 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM, KS>), 2) void k_mx
         reinterpret_cast<v4f*>(src)[0] = y[0];
         reinterpret_cast<v4f*>(src)[1] = y[1];
       }
-      product_store8(p, row, ch, src, pre[(EARLY ? b * PASSES : 0) + r]);
+      product_store8<STREAM>(p, row, ch, src, pre[(EARLY ? b * PASSES : 0) + r]);
     }
   }
 }
@@ -805,6 +810,23 @@ static bool product_near(const ProductArgs& p) {
   return (uint64_t)std::max(std::max(p.a_ld, p.b_ld), std::max(p.as_ld, p.bs_ld)) * 256 < (1ull << 32);
 }
 
+// Streaming or ordinary stores of a product's output.  Streaming ones keep the write-back L2 out of the way, but an L2 that they pass
+// cannot join parts of a 128-byte line: an fp32 store of 8 channels is two halves of 16 of every 32 bytes, and rows that are not whole
+// lines begin and end inside one.  us streaming | ordinary:
+//   fp16, tiled kernels: 8192 x 8192 x 2048 94 | 111, 8192 x 8190 x 2048 110 | 125, 20000 x 1000 x 1000 33.8 | 34.8, 100000 x 128 x 300
+//     14.0 | 19.9, 100000 x 100 x 300 17.2 | 20.3: streaming;
+//   fp32, tiles of 128 and 256: 8192 x 8192 x 2048 167 | 129, 20000 x 1024 x 1000 53 | 41, 20000 x 500 x 1000 33.7 | 32.8: ordinary;
+//   fp32, tiles of 64: 100000 x 128 x 300 17.9 | 25.5, 2000 x 1024 x 300 5.6 | 6.1, but 2000 x 1000 x 300 8.1 | 6.5: by whole lines;
+//   quantised in the same launch, fp16: up to 4 blocks 123646 x 256 x 128 22.6 | 28.5, but 123646 x 250 x 128 46.5 | 34.0 and 20000 x
+//     1000 x 100 25.8 | 22.6: by whole lines; more blocks 60000 x 250 x 250 24.9 | 28.3: streaming;
+//   quantised in the same launch, fp32: 123646 x 250 x 128 92 | 47, 60000 x 250 x 250 41.8 | 33.8: by whole lines; with them 60000 x 128 x
+//     256 17.6 | 21.1, 123646 x 96 x 64 17.9 | 21.5, but in the wide tiles of more than 128 channels 123646 x 256 x 128 53 | 41 and
+//     20000 x 512 x 100 20.3 | 17.1 (5000 x 1024 x 128, which the L2 holds, 10.2 | 11.3).
+static bool whole_lines(const ProductArgs& p) {
+  const size_t size = p.out_fp32 ? 4 : 2;
+  return ((uintptr_t)p.out | (size_t)p.out_ld * size | (size_t)p.n * size) % 128 == 0;
+}
+
 template <int BN, int BM, int TN, int TM, int KS>
 static int launch_product(const ProductArgs& p, const scn_mx_product_io& io, hipStream_t stream) {
   using T = ProductTile<BN, BM, TN, TM, KS>;
@@ -815,8 +837,12 @@ static int launch_product(const ProductArgs& p, const scn_mx_product_io& io, hip
               p.m, p.n);
   if (int rc = product_start(p, io, stream)) return rc;
   const uint32_t stages = (p.kb + 7) / 8;
-  hipLaunchKernelGGL((k_mx_product_lds<BN, BM, TN, TM, KS>), dim3((unsigned)((tn * tm + 7) / 8 * 8)), dim3((unsigned)threads),
-                     KS * T::lds(std::min(T::share(stages), stages)), stream, p, (uint32_t)tn, (uint32_t)tm);
+  const auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((tn * tm + 7) / 8 * 8)), dim3((unsigned)threads),
+                       KS * T::lds(std::min(T::share(stages), stages)), stream, p, (uint32_t)tn, (uint32_t)tm);
+  };
+  if (!p.out_fp32 || (BN == 64 && whole_lines(p))) launch(k_mx_product_lds<BN, BM, TN, TM, KS, true>);
+  else launch(k_mx_product_lds<BN, BM, TN, TM, KS, false>);
   return SCN_OK;
 }
 
@@ -834,7 +860,7 @@ struct FusedTile {
   static constexpr int LDS = WC + WN * 64 * P * 16 > STORE ? WC + WN * 64 * P * 16 : STORE;
 };
 
-template <int AT, int WN, int P>
+template <int AT, int WN, int P, bool STREAM>
 __global__ __launch_bounds__((64 * FusedTile<AT, WN, P>::NW)) void k_mx_product_fused(const ProductArgs p) {
   using F = FusedTile<AT, WN, P>;
   typedef typename MxIn<AT>::T T;
@@ -963,27 +989,34 @@ __global__ __launch_bounds__((64 * FusedTile<AT, WN, P>::NW)) void k_mx_product_
 #pragma unroll
     for (int r = 0; r < PASSES; ++r) {
       const uint32_t row = row0 + (b * PASSES + r) * RPP;
-      if (row < m && ch < p.n) product_store8(p, row, ch, buf + (r * RPP + lane / LPR) * F::PAD + (lane % LPR) * 8, pre[b * PASSES + r]);
+      if (row < m && ch < p.n)
+        product_store8<STREAM>(p, row, ch, buf + (r * RPP + lane / LPR) * F::PAD + (lane % LPR) * 8, pre[b * PASSES + r]);
     }
   }
 }
 
-template <int AT, int WN>
+template <int AT, int WN, bool STREAM>
 static void launch_fused(const ProductArgs& p, hipStream_t stream) {
   const auto launch = [&](auto kernel, uint32_t rows, uint32_t waves) {
     hipLaunchKernelGGL(kernel, dim3(ceil_div(p.m, rows), ceil_div(p.n, 64u * WN)), dim3(64 * waves), 0, stream, p);
   };
-  if (p.kb <= 2) launch(k_mx_product_fused<AT, WN, 2>, FusedTile<AT, WN, 2>::BM, FusedTile<AT, WN, 2>::NW);
-  else if (p.kb <= 4) launch(k_mx_product_fused<AT, WN, 4>, FusedTile<AT, WN, 4>::BM, FusedTile<AT, WN, 4>::NW);
-  else launch(k_mx_product_fused<AT, WN, 8>, FusedTile<AT, WN, 8>::BM, FusedTile<AT, WN, 8>::NW);
+  if (p.kb <= 2) launch(k_mx_product_fused<AT, WN, 2, STREAM>, FusedTile<AT, WN, 2>::BM, FusedTile<AT, WN, 2>::NW);
+  else if (p.kb <= 4) launch(k_mx_product_fused<AT, WN, 4, STREAM>, FusedTile<AT, WN, 4>::BM, FusedTile<AT, WN, 4>::NW);
+  else launch(k_mx_product_fused<AT, WN, 8, STREAM>, FusedTile<AT, WN, 8>::BM, FusedTile<AT, WN, 8>::NW);
+}
+template <int AT, bool STREAM>
+static void launch_fused(const ProductArgs& p, hipStream_t stream) {
+  if (p.n <= 64) launch_fused<AT, 1, STREAM>(p, stream);
+  else if (p.n <= 128) launch_fused<AT, 2, STREAM>(p, stream);
+  else launch_fused<AT, 4, STREAM>(p, stream);
 }
 template <int AT>
 static int launch_fused(const ProductArgs& p, const scn_mx_product_io& io, hipStream_t stream) {
   SCN_REQUIRE((uint64_t)p.b_ld * 256 < (1ull << 32), SCN_ERR_UNSUPPORTED, "mx_product: rows more than 16 MB apart");
   if (int rc = product_start(p, io, stream)) return rc;
-  if (p.n <= 64) launch_fused<AT, 1>(p, stream);
-  else if (p.n <= 128) launch_fused<AT, 2>(p, stream);
-  else launch_fused<AT, 4>(p, stream);
+  const bool wide = p.n > 128 && p.kb <= 4 && (uint64_t)p.m * p.n > (8u << 20);
+  if (p.out_fp32 ? whole_lines(p) && !wide : whole_lines(p) || p.kb > 4) launch_fused<AT, true>(p, stream);
+  else launch_fused<AT, false>(p, stream);
   return SCN_OK;
 }
 

@@ -58,7 +58,7 @@ inline bool mx_overlap(const MxSpan& a, const MxSpan& b) {
   if (pa + (a.rows - 1) * a.ld + a.width <= pb || pb + (b.rows - 1) * b.ld + b.width <= pa) return false;
   const uint64_t ld = a.rows > 1 ? a.ld : b.ld;   // (a single row has no stride of its own)
   if ((a.rows > 1 && b.rows > 1 && a.ld != b.ld) || (a.rows == 1 && b.rows == 1) || ld == 0) return true;
-  const uint64_t d = (uint64_t)(pb >= pa ? (pb - pa) % ld : (ld - (pa - pb) % ld) % ld);   // where b's rows start behind a's
+  const uint64_t gap = (uint64_t)(pb >= pa ? pb - pa : pa - pb) % ld, d = pb >= pa || gap == 0 ? gap : ld - gap;   // where b's rows start behind a's
   return d < a.width || d + b.width > ld;
 }
 

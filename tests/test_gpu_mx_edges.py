@@ -326,3 +326,28 @@ def test_convolutions_add_every_neighbour_once(cin, cout, n, bound, ks):
     capi.check(capi.lib().scn_conv_forward(conv._h, rb._h, C.byref(io), torch.cuda.current_stream().cuda_stream))
     y, _ = R.convolution(xv, w, None, table)
     assert np.array_equal(acc.double().cpu().numpy(), y)
+
+
+# tiles of 64, 128 and 256, k in parts, rows quantised in the same launch (narrow, wide, long, beyond the caches)
+@pytest.mark.parametrize("m, n, k, x", [(200, 128, 300, "mx"), (2100, 2304, 600, "mx"), (4200, 4352, 300, "mx"), (70, 128, 4000, "mx"), (200, 64, 64, "fp16"),
+                                        (300, 1024, 128, "fp16"), (100, 256, 256, "fp32"), (33000, 256, 100, "fp16")])
+@pytest.mark.parametrize("out_dtype", [torch.float16, torch.float32])
+def test_product_results_in_rows_of_whole_lines_and_others(m, n, k, x, out_dtype):
+    """How results are stored depends on whether their rows are whole 128-byte lines; what is stored does not, nor does
+    anything else get written."""
+    mx = _mx()
+    torch.manual_seed(m)
+    w, a = mx.quantize_rows(torch.randn(n, k, device=DEV)), torch.randn(m, k, device=DEV)
+    a = mx.quantize_rows(a) if x == "mx" else a.to(torch.float16 if x == "fp16" else torch.float32)
+    res = torch.randn(m, n, device=DEV).half()
+    want = mx.product(a, w, out_dtype=out_dtype, relu=True, residual=res)
+    av = mx.dequantize_rows(a if x == "mx" else mx.quantize_rows(a), torch.float32)[:64].double()
+    y, mag = R.product(av.cpu().numpy(), mx.dequantize_rows(w, torch.float32).double().cpu().numpy(), None, True, res[:64].double().cpu().numpy())
+    R.within(want[:64].double().cpu().numpy(), y, R.tolerance(y, mag, k, 2.0 ** -11 if out_dtype == torch.float16 else 2.0 ** -24))
+    for lead, extra in ((0, 32 // want.element_size() * 4), (0, 8), (64 // want.element_size(), 0), (1, 0), (3, 5)):
+        flat = torch.full((lead + m * (n + extra) + 64,), 9.0, dtype=out_dtype, device=DEV)
+        out = flat[lead:lead + m * (n + extra)].view(m, n + extra)[:, :n]
+        mx.product(a, w, relu=True, residual=res, out=out)
+        assert torch.equal(out, want), (lead, extra)
+        out.fill_(9)
+        assert (flat == 9).all(), (lead, extra)
