@@ -96,6 +96,7 @@ struct ConvMxStage {
   static constexpr int PAD = 32 * MT + 4;                        // floats per row of the store buffer
   static constexpr int WAVE = 2 * BYTES > 32 * PAD * 4 ? 2 * BYTES : 32 * PAD * 4;
   static constexpr int LDS = RING + W * WAVE;
+  static constexpr int PER_CU = 160 * 1024 / ((LDS + 1279) / 1280 * 1280);   // workgroups whose LDS a CU holds (handed out in 1,280 bytes)
 };
 
 // 64 x 16 bytes to LDS, lane l's to base + 16 l: in assembly, because the compiler would order its own LDS
@@ -367,24 +368,30 @@ static void launch_gather(ConvArgs& a, const uint8_t* ws, int mtiles, hipStream_
                      dim3(64 * W), 0, stream, a, ws, mtiles);
 }
 
-// Waves per 64 rows.  Few tiles are bound by the latency of a wave's chain of stages, which more waves shorten; where the tiles
-// of one wave just fill the GPU (12 per CU), one has the fewest instructions; beyond that two balance better.  us with 1 / 2 / 4
-// waves: 20,000 rows 64 -> 64 14.2 / 10.2 / 7.9, 120,000 rows 22.2 / 25.4 / 25.3, 260,000 rows 45.0 / 40.5 / 45.1; with 128
-// output channels (twice the work per wave) with 2 / 4: 20,000 rows 128 -> 128 18.6 / 15.5, 48,460 rows 64 -> 128 15.8 / 18.9,
-// 150,000 rows 128 -> 128 59.3 / 61.7.
+// Waves per 64 rows.  Few tiles are bound by the latency of a wave's chain of stages, which more waves shorten.  More of them take
+// two waves while all tiles run at once, then one wave while those do, then two again, which balance better over several rounds.
+// LDS limits how many run: 9 one-wave or 6 two-wave workgroups a CU at 32 and 64 -> 64 channels (147,456 and 98,304 rows; registers
+// would allow 16 waves), 10 or 6 at 16 -> 16, 9 or 5 at 128 -> 64.  us with 1 / 2 / 4 waves, 64 -> 64: 20,000 rows 14.6 / 10.6 / 8.4, 50,000
+// 17.1 / 12.6 / 14.5, 80,000 21.4 / 16.2 / 18.4, 95,000 22.2 / 17.6 / 20.0, 110,000 23.3 / 25.6 / 24.1, 142,000 26.2 / 27.1 / 27.1, 163,000 37.9 /
+// 28.3 / 31.3, 196,000 39.5 / 34.8 / 34.5, 260,000 43.7 / 39.4 / 44.9; 16 -> 16: 95,000 13.6 / 10.3 / 13.1, 163,000 16.2 / 17.8 / 19.5, 190,000
+// 25.0 / 18.6 / 21.7; 128 -> 64: 80,000 25.1 / 20.9 / 22.9, 95,000 26.5 / 29.2 / 25.0; with 128 output channels (twice the work per wave)
+// with 2 / 4: 20,000 rows 128 -> 128 18.7 / 15.7, 48,460 rows 64 -> 128 17.2 / 20.1, 150,000 rows 128 -> 128 57.0 / 60.9.
 // The choice follows the bound of the row count, never the count or what an earlier forward had: the order of the sums, and
 // so their last bit, depends on it.
+template <int BPR, int MT, int MODE>
+static void launch_waves(ConvArgs& a, const uint8_t* ws, int mtiles, hipStream_t stream) {
+  const uint64_t tiles = ((uint64_t)a.n_bound + 63) / 64;
+  if (a.n_bound <= 32768) return launch_gather<BPR, MT, 4, MODE>(a, ws, mtiles, stream);
+  if constexpr (MT <= 2)
+    if (tiles > 256u * ConvMxStage<BPR, MT, 2>::PER_CU && tiles <= 256u * ConvMxStage<BPR, MT, 1>::PER_CU)
+      return launch_gather<BPR, MT, 1, MODE>(a, ws, mtiles, stream);
+  launch_gather<BPR, MT, 2, MODE>(a, ws, mtiles, stream);
+}
 template <int BPR, int MODE>
 static void launch_gather(ConvArgs& a, const uint8_t* ws, int mtiles, hipStream_t stream) {
-  const int waves = a.n_bound <= 32768 ? 4 : a.n_bound <= 65536 || a.n_bound > 196608 || mtiles > 2 ? 2 : 1;
-  if (mtiles > 2 && waves == 4) launch_gather<BPR, 4, 4, MODE>(a, ws, mtiles, stream);
-  else if (mtiles > 2) launch_gather<BPR, 4, 2, MODE>(a, ws, mtiles, stream);
-  else if (mtiles == 2 && waves == 4) launch_gather<BPR, 2, 4, MODE>(a, ws, mtiles, stream);
-  else if (mtiles == 2 && waves == 2) launch_gather<BPR, 2, 2, MODE>(a, ws, mtiles, stream);
-  else if (mtiles == 2) launch_gather<BPR, 2, 1, MODE>(a, ws, mtiles, stream);
-  else if (waves == 4) launch_gather<BPR, 1, 4, MODE>(a, ws, mtiles, stream);
-  else if (waves == 2) launch_gather<BPR, 1, 2, MODE>(a, ws, mtiles, stream);
-  else launch_gather<BPR, 1, 1, MODE>(a, ws, mtiles, stream);
+  if (mtiles > 2) launch_waves<BPR, 4, MODE>(a, ws, mtiles, stream);
+  else if (mtiles == 2) launch_waves<BPR, 2, MODE>(a, ws, mtiles, stream);
+  else launch_waves<BPR, 1, MODE>(a, ws, mtiles, stream);
 }
 
 template <int BPR>

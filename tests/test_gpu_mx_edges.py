@@ -351,3 +351,31 @@ def test_product_results_in_rows_of_whole_lines_and_others(m, n, k, x, out_dtype
         assert torch.equal(out, want), (lead, extra)
         out.fill_(9)
         assert (flat == 9).all(), (lead, extra)
+
+
+@pytest.mark.parametrize("cin, cout", [(16, 16), (64, 64), (96, 48)])
+def test_convolutions_of_medium_and_large_bounds_share_a_tile_between_two_waves(cin, cout):
+    """The bound of the row count chooses how many waves share a tile, and so the order of the sums: these bounds have the
+    same one.  (Blocks of very different strength: the sums have to be rounded.)"""
+    import ctypes as C
+    mx = _mx()
+    rng = np.random.default_rng(cin)
+    n, kv = 900, 27
+    coords = np.stack(np.unravel_index(np.sort(rng.choice(9 * 12 * 12, n, replace=False)), (9, 12, 12)), 1)
+    x = (rng.standard_normal((n, cin)) * np.exp2(rng.integers(-8, 9, (n, 1)))).astype(np.float16)
+    conv = mx.Conv((rng.standard_normal((cout, 3, 3, 3, cin)) * np.exp2(rng.integers(-8, 9, (1, 3, 3, 3, 1)))).astype(np.float16))
+    q = mx.quantize_rows(torch.from_numpy(x).to(DEV))
+    sums = []
+    for bound in (40000, 66000, 98304, 163841, 190000, 200000):
+        idx = torch.zeros((bound, 4), dtype=torch.int32, device=DEV)
+        idx[:n, 1:] = torch.from_numpy(coords.astype(np.int32)).to(DEV)
+        rb = mx.Rulebook(bound, bound, kv)
+        rb.build_subm(idx, (9, 12, 12), (3, 3, 3), num=torch.tensor([n], dtype=torch.int32, device=DEV))
+        acc = torch.full((n, cout), 7.0, device=DEV)
+        out = torch.empty((n, cout), dtype=torch.float16, device=DEV)
+        io = capi.ConvIO()
+        io.x_dev, io.x_ld, io.out_dtype = q.codes_ptr, q.codes_ld, capi.DTYPE_FP16
+        io.out_dev, io.out_ld, io.acc_dev = out.data_ptr(), cout, acc.data_ptr()
+        capi.check(capi.lib().scn_conv_forward(conv._h, rb._h, C.byref(io), torch.cuda.current_stream().cuda_stream))
+        sums.append(acc)
+        assert torch.equal(acc, sums[0]), bound
