@@ -778,12 +778,14 @@ __global__ __launch_bounds__((kProductThreads<BN, BM, TN, TM, KS>), 2) void k_mx
   }
 }
 
+static size_t product_workspace(uint32_t m, uint32_t n, uint32_t k);   // 0: rows of fp16 / fp32 need none
+
 // What comes in front of a product's launch, once its kernel has taken the sizes: no operand lies where the call writes, and rows
 // that go through the workspace (p.a is that then) are quantised into it.
 static int product_start(const ProductArgs& p, const scn_mx_product_io& io, hipStream_t stream) {
   const auto size = [](int dtype) -> uint64_t { return dtype == SCN_DTYPE_FP32 ? 4 : 2; };
   const uint64_t codes = (uint64_t)p.kb * kMxBlockBytes, scales = mx_scale_bytes(p.k);
-  const bool mx = io.a_dtype == SCN_DTYPE_MXFP4, quantise = p.a != io.a_dev;
+  const bool mx = io.a_dtype == SCN_DTYPE_MXFP4, quantise = !mx && product_workspace(io.m, io.n, io.k) != 0;
   const MxSpan out{io.out_dev, io.m, io.n * size(io.out_dtype), io.out_ld * size(io.out_dtype)},
       ws{quantise ? p.a : nullptr, 1, (uint64_t)io.m * p.a_ld, 0},
       res{io.res_dev, io.m, io.n * size(io.res_dtype), io.res_ld * size(io.res_dtype)};

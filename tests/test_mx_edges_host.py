@@ -44,7 +44,7 @@ OVER = [dict(out_dev=GOOD + 39 * 176 + 158),                              # the 
         dict(out_dev=4 * GOOD + 36),                                      # columns that run into the next row's
         dict(out_dev=6 * GOOD), dict(out_dev=GOOD + 100, out_ld=88),      # (stride of the rows, columns of them)
         dict(FP16_ROWS, out_dev=GOOD + 2), dict(FP16_ROWS, out_dev=GOOD + 39 * 640 + 638), dict(FP16_ROWS, out_dev=GOOD, m=3),
-        dict(FP16_ROWS, workspace_dev=GOOD + 16), dict(FP16_ROWS, workspace_dev=2 * GOOD - 16), dict(FP16_ROWS, workspace_dev=3 * GOOD + 80),
+        dict(FP16_ROWS, workspace_dev=GOOD), dict(FP16_ROWS, workspace_dev=GOOD + 16), dict(FP16_ROWS, workspace_dev=2 * GOOD - 16), dict(FP16_ROWS, workspace_dev=3 * GOOD + 80),
         dict(FP16_ROWS, workspace_dev=4 * GOOD + 48), dict(FP16_ROWS, workspace_dev=5 * GOOD - 7024), dict(FP16_ROWS, workspace_dev=6 * GOOD - 16)]
 
 
